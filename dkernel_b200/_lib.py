@@ -92,6 +92,49 @@ class XchgParams(C.Structure):
                 + [("part_o", _vp), ("part_lse", _vp), ("nsplit", _i32)])
 
 
+class PagedStepParams(C.Structure):
+    _fields_ = ([("block_tables", _vp), ("table_stride", _i64)]
+                + [(n, _vp) for n in ("page_counts", "free_pages", "num_free", "context_lens", "new_lens", "tree_mask",
+                                      "cu_seqlen_q", "seqlens", "slots", "positions", "short_pages")]
+                + [(n, _i32) for n in ("batch", "max_pages", "free_capacity", "page_size", "max_tokens")])
+
+
+class PagedWriteParams(C.Structure):
+    _fields_ = ([("k", _vp), ("v", _vp)]
+                + [(n, _i64) for n in ("k_st", "k_sh", "v_st", "v_sh")]
+                + [("k_cache", _vp), ("v_cache", _vp)]
+                + [(n, _i64) for n in ("kc_sp", "kc_ss", "kc_sh", "vc_sp", "vc_ss", "vc_sh")]
+                + [("slots", _vp)]
+                + [(n, _i32) for n in ("tokens", "hkv", "d", "page_size", "num_pages", "dtype", "cache_dtype")]
+                + [("k_scale", _f32), ("v_scale", _f32)])
+
+
+class PagedParams(C.Structure):
+    _fields_ = ([("q", _vp), ("o", _vp), ("lse", _vp)]
+                + [(n, _i64) for n in ("q_st", "q_sh", "o_st", "o_sh", "lse_sh")]
+                + [("k_cache", _vp), ("v_cache", _vp)]
+                + [(n, _i64) for n in ("kc_sp", "kc_ss", "kc_sh", "vc_sp", "vc_ss", "vc_sh")]
+                + [("block_tables", _vp), ("table_stride", _i64)]
+                + [(n, _vp) for n in ("seqlens", "cu_q", "tree_mask", "crow", "col")]
+                + [("crow_sh", _i64), ("col_sh", _i64)]
+                + [(n, _i32) for n in ("h_pat", "n_rows", "block_size", "heads_share", "batch", "hq", "hkv", "d",
+                                       "total_q", "max_pages", "page_size", "num_pages", "dtype", "kv_dtype")]
+                + [(n, _f32) for n in ("sm_scale", "k_scale", "v_scale")] + [("impl", _i32), ("ws", _vp)])
+
+
+class PagedCommitParams(C.Structure):
+    _fields_ = ([("k_cache", _vp), ("v_cache", _vp)]
+                + [(n, _i64) for n in ("kc_sp", "kc_ss", "kc_sh", "vc_sp", "vc_ss", "vc_sh")]
+                + [("block_tables", _vp), ("table_stride", _i64)]
+                + [(n, _vp) for n in ("context_lens", "cu_q", "accepted", "tree_mask", "new_context_lens")]
+                + [(n, _i32) for n in ("batch", "hkv", "d", "total_q", "max_pages", "page_size", "num_pages",
+                                       "cache_dtype")])
+
+
+PAGED_STEP_PACK, PAGED_WRITE_PACK = _packer(PagedStepParams), _packer(PagedWriteParams)
+PAGED_PACK, PAGED_COMMIT_PACK = _packer(PagedParams), _packer(PagedCommitParams)
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "bsa_abi_version": (_i32, []),
@@ -114,6 +157,12 @@ EXPORTS = {
     "bsa_set_wait_status_mirror": (_i32, [_vp]),
     "bsa_selftest_wait_timeout": (_i32, [C.c_uint32, _vp]),
     "bsa_fwd_why_not_sm100": (C.c_char_p, [C.POINTER(FwdParams)]),
+    "bsa_paged_step": (_i32, [C.POINTER(PagedStepParams), _vp]),
+    "bsa_paged_write": (_i32, [C.POINTER(PagedWriteParams), _vp]),
+    "bsa_paged_workspace_bytes": (C.c_size_t, [C.POINTER(PagedParams)]),
+    "bsa_paged_fwd": (_i32, [C.POINTER(PagedParams), _vp]),
+    "bsa_paged_why_not_sm100": (C.c_char_p, [C.POINTER(PagedParams)]),
+    "bsa_paged_commit": (_i32, [C.POINTER(PagedCommitParams), _vp]),
 }
 
 _lib = None

@@ -1,0 +1,456 @@
+// Paged K/V cache: a step's bookkeeping, cache writes, committed branches, and the CUDA-core form of the
+// attention (the tcgen05 form is in paged_sm100.cu).  Semantics: include/bsa.h.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace bsa {
+namespace {
+
+// ------------------------------------------------------------------ a step's tables
+// One cluster does everything: each CTA scans all requests (a few loads per thread; a scan spread over CTAs
+// would cost the exchange of its sums instead) and keeps offsets in shared memory; pages and tokens are then
+// shared out.  The barrier between pushing surplus pages and popping missing ones is the cluster's own, so a
+// step is one launch.
+constexpr int kStepThreads = 1024;
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// inclusive scan over the block's threads; total = sum of all
+__device__ __forceinline__ long long block_scan(long long x, long long* warp_sums, long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += up;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    long long s = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += up;
+    }
+    warp_sums[lane] = s;
+  }
+  __syncthreads();
+  x += warp ? warp_sums[warp - 1] : 0;
+  *total = warp_sums[kStepThreads / 32 - 1];
+  __syncthreads();
+  return x;
+}
+
+__global__ void __launch_bounds__(kStepThreads) paged_step_kernel(bsa_paged_step_params p, int ctas) {
+  extern __shared__ int step_smem[];
+  __shared__ long long warp_sums[32];
+  const int B = p.batch, P = p.page_size, T = p.max_tokens, W = p.max_pages;
+  int* cu = step_smem;            // [B + 1]
+  int* held = cu + B + 1;         // [B] pages before the step
+  int* target = held + B;         // [B] pages after it
+  int* off = target + B;          // [B] first push (target < held) or first pop
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = blockIdx.x;
+
+  const int n_free = min(max(__ldg(p.num_free), 0), p.free_capacity);
+  long long new_before = 0, moved_before = 0;
+  if (tid == 0) cu[0] = 0;
+  for (int b0 = 0; b0 < B; b0 += kStepThreads) {
+    const int b = b0 + tid;
+    const int want = b < B ? max(__ldg(p.new_lens + b), 0) : 0;
+    const int ctx = b < B ? max(__ldg(p.context_lens + b), 0) : 0;
+    const int h = b < B ? min(max(__ldg(p.page_counts + b), 0), W) : 0;
+    long long total;
+    const long long incl = block_scan(want, warp_sums, &total) + new_before;
+    const int c1 = (int)min(incl, (long long)T), c0 = (int)min(incl - want, (long long)T);
+    const long long len = (long long)ctx + (c1 - c0);
+    const int tg = b < B ? (int)min((len + P - 1) / P, (long long)W) : 0;
+    // pushes in the low half, pops in the high half: W * B < 2^31 is checked by the host
+    const long long moved = tg < h ? (long long)(h - tg) : (long long)(tg - h) << 32;
+    long long total2;
+    const long long mincl = block_scan(moved, warp_sums, &total2) + moved_before;
+    if (b < B) {
+      cu[b + 1] = c1;
+      held[b] = h;
+      target[b] = tg;
+      off[b] = tg < h ? (int)((mincl - moved) & 0xffffffffll) : (int)((mincl - moved) >> 32);
+      if (rank == 0) {
+        p.cu_seqlen_q[b + 1] = c1;
+        p.seqlens[b] = (int)min(len, 0x7fffffffll);
+      }
+    }
+    new_before += total;
+    moved_before += total2;
+  }
+  __syncthreads();
+  const int pushes = (int)(moved_before & 0xffffffffll), pops = (int)(moved_before >> 32);
+  if (rank == 0 && tid == 0) p.cu_seqlen_q[0] = 0;
+
+  // surplus pages go on the stack, a warp per request
+  const int warps = ctas * (kStepThreads / 32);
+  if (pushes)
+    for (int b = rank * (kStepThreads / 32) + warp; b < B; b += warps)
+      for (int i = target[b] + lane; i < held[b]; i += 32) {
+        const long long at = (long long)n_free + off[b] + i - target[b];
+        int32_t* entry = p.block_tables + (int64_t)b * p.table_stride + i;
+        if (at < p.free_capacity) p.free_pages[at] = *entry;
+        *entry = -1;
+      }
+  if (ctas > 1) cluster_sync_all(); else __syncthreads();
+
+  const int avail = (int)min((long long)n_free + pushes, (long long)p.free_capacity);
+  // page `nth` (in the order of request and page) of the missing ones; not through the read-only cache, the
+  // stack has just been written
+  auto popped = [&](int nth) { return nth < avail ? *(volatile int32_t*)(p.free_pages + (avail - 1 - nth)) : -1; };
+  if (pops)
+    for (int b = rank * (kStepThreads / 32) + warp; b < B; b += warps)
+      for (int i = held[b] + lane; i < target[b]; i += 32)
+        p.block_tables[(int64_t)b * p.table_stride + i] = popped(off[b] + i - held[b]);
+  if (rank == 0) {
+    for (int b = tid; b < B; b += kStepThreads) {
+      const int h = held[b], tg = target[b];
+      if (tg != h) p.page_counts[b] = tg < h ? tg : h + min(max(avail - off[b], 0), tg - h);
+    }
+    if (tid == 0) {
+      *p.num_free = max(avail - pops, 0);
+      *p.short_pages = max(pops - avail, 0);
+    }
+  }
+
+  const int real = cu[B];
+  for (int t = rank * kStepThreads + tid; t < T; t += ctas * kStepThreads) {
+    long long slot = -1;
+    int pos = 0;
+    if (t < real) {
+      int lo = 0, hi = B;                       // cu[lo] <= t < cu[lo + 1]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid] <= t) lo = mid; else hi = mid;
+      }
+      const int b = lo, i = t - cu[b], n = cu[b + 1] - cu[b];
+      const long long ctx = max(__ldg(p.context_lens + b), 0), at = ctx + i, pi = at / P;
+      if (pi < target[b]) {
+        const int pg = pi < held[b] ? *(volatile int32_t*)(p.block_tables + (int64_t)b * p.table_stride + pi)
+                                    : popped(off[b] + (int)pi - held[b]);
+        if (pg >= 0) slot = (long long)pg * P + at % P;
+      }
+      int depth = i;
+      if (p.tree_mask) {
+        const uint64_t word = (uint64_t)__ldg(p.tree_mask + t) & low_bits(n);
+        depth = draft_depth(word, i);
+      }
+      pos = (int)min(ctx + depth, 0x7fffffffll);
+    }
+    p.slots[t] = slot;
+    p.positions[t] = pos;
+  }
+  if (ctas > 1) cluster_sync_all();   // no CTA leaves while another may still need the cluster's barrier
+}
+
+// ------------------------------------------------------------------ cache writes
+template <typename T> __device__ __forceinline__ uint8_t to_e4m3(T x, float scale) {
+  // a true division: k / scale decides ties, k * (1 / scale) would not
+  return (uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(Elem<T>::to_f(x), scale), __NV_SATFINITE, __NV_E4M3);
+}
+
+// Both caches in one grid: blockIdx.y = 0 for K, 1 for V.  A thread moves VEC elements (16 bytes of the input
+// where everything is aligned, else one element); consecutive threads are consecutive in (token, head, dim).
+template <typename T, typename C, int VEC>
+__global__ void __launch_bounds__(256) paged_write_kernel(bsa_paged_write_params p) {
+  const bool is_v = blockIdx.y != 0;
+  const T* src = static_cast<const T*>(is_v ? p.v : p.k);
+  C* dst = static_cast<C*>(is_v ? p.v_cache : p.k_cache);
+  const int64_t st = is_v ? p.v_st : p.k_st, sh = is_v ? p.v_sh : p.k_sh;
+  const int64_t cp = is_v ? p.vc_sp : p.kc_sp, cs = is_v ? p.vc_ss : p.kc_ss, ch = is_v ? p.vc_sh : p.kc_sh;
+  const float scale = is_v ? p.v_scale : p.k_scale;
+  const int pieces = p.d / VEC;
+  const int64_t per_token = (int64_t)p.hkv * pieces, total = per_token * p.tokens;
+  const int64_t slots = (int64_t)p.num_pages * p.page_size;
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < total; x += (int64_t)gridDim.x * 256) {
+    const int t = (int)(x / per_token), rem = (int)(x - t * per_token), h = rem / pieces, e = (rem - h * pieces) * VEC;
+    const int64_t slot = __ldg(p.slots + t);
+    if (slot < 0 || slot >= slots) continue;
+    const T* s = src + (int64_t)t * st + (int64_t)h * sh + e;
+    const int64_t page = slot / p.page_size;
+    C* o = dst + page * cp + (slot - page * p.page_size) * cs + (int64_t)h * ch + e;
+    if constexpr (VEC == 1) {
+      if constexpr (sizeof(C) == 1) *o = to_e4m3(*s, scale);
+      else *o = *s;
+    } else {
+      uint4 in = *reinterpret_cast<const uint4*>(s);
+      if constexpr (sizeof(C) == 1) {
+        const T* y = reinterpret_cast<const T*>(&in);
+        alignas(16) uint8_t out[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = to_e4m3(y[i], scale);
+        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(out);
+        else *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(out);
+      } else {
+        *reinterpret_cast<uint4*>(o) = in;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ committed branches
+// CTA (x, request): its threads own V-byte pieces of a token's K and V rows.  Draft numbers on a branch ascend,
+// so the r-th is at least r: token L + r is written when every branch token that was there has been read.
+template <typename V>
+__global__ void __launch_bounds__(256) paged_commit_kernel(bsa_paged_commit_params p, int elem_bytes) {
+  const int b = blockIdx.y;
+  const int t0 = min(max(__ldg(p.cu_q + b), 0), p.total_q);
+  const int n = min(max(__ldg(p.cu_q + b + 1) - t0, 0), p.total_q - t0);
+  const int a = __ldg(p.accepted + b), L = max(__ldg(p.context_lens + b), 0);
+  const bool any = a >= 0 && a < n && (!p.tree_mask || a < 64);
+  uint64_t word = 0;
+  if (any && p.tree_mask) {
+    word = ((uint64_t)__ldg(p.tree_mask + t0 + a) & low_bits(n)) | 1ull << a;
+  }
+  const int count = !any ? 0 : p.tree_mask ? __popcll(word) : a + 1;
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.new_context_lens[b] = L + count;
+  if (!p.tree_mask || !any) return;   // a chain is in place already
+  const int stay = __ffsll((long long)~word) - 1;   // the first drafts 0, 1, ... are, too (-1: all 64)
+  if (stay < 0 || stay >= count) return;
+  const int32_t* table = p.block_tables + (int64_t)b * p.table_stride;
+  const int pieces = p.d * elem_bytes / (int)sizeof(V), per_cache = p.hkv * pieces;
+  for (int x = blockIdx.x * 256 + threadIdx.x; x < 2 * per_cache; x += gridDim.x * 256) {
+    const bool is_v = x >= per_cache;
+    const int y = is_v ? x - per_cache : x, h = y / pieces, c = y - h * pieces;
+    char* base = static_cast<char*>(is_v ? p.v_cache : p.k_cache);
+    const int64_t sp = is_v ? p.vc_sp : p.kc_sp, ss = is_v ? p.vc_ss : p.kc_ss, sh = is_v ? p.vc_sh : p.kc_sh;
+    auto place = [&](int at) -> V* {
+      const int pg = page_of(table, at / p.page_size, p.max_pages, p.num_pages);
+      if (pg < 0) return nullptr;
+      return reinterpret_cast<V*>(base + ((int64_t)pg * sp + (int64_t)(at % p.page_size) * ss + (int64_t)h * sh) * elem_bytes) + c;
+    };
+    uint64_t left = word & ~low_bits(stay);
+    int r = stay;
+    while (left) {
+      // four at a time: their loads are in flight together
+      V val[4];
+      const V* src[4];
+      int m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        src[i] = nullptr;
+        if (!left) continue;
+        src[i] = place(L + __ffsll((long long)left) - 1);
+        left &= left - 1;
+        if (src[i]) val[i] = *src[i];
+        ++m;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= m) continue;
+        V* dst = place(L + r + i);
+        if (src[i] && dst) *dst = val[i];
+      }
+      r += m;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ attention on the CUDA cores
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) paged_rows_kernel(bsa_paged_params p) {
+  const int64_t x = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (x >= (int64_t)p.total_q * p.hq) return;
+  const int t = (int)(x / p.hq), h = (int)(x % p.hq);
+  int b = t;
+  if (p.cu_q) {
+    if (t < __ldg(p.cu_q) || t >= __ldg(p.cu_q + p.batch)) return;
+    int lo = 0, hi = p.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(p.cu_q + mid) <= t) lo = mid; else hi = mid;
+    }
+    b = lo;
+  }
+  if (b >= p.batch) return;
+  const PagedRequest r = paged_request(p, b);
+  if (t - r.t0 >= r.n) return;
+  paged_row<T, C>(p, b, r, t - r.t0, h, lane);
+}
+
+bool known_dtype(int t) { return t == BSA_F16 || t == BSA_BF16 || t == BSA_F32; }
+
+int validate_paged(const bsa_paged_params* p, const char* who) {
+  BSA_CHECK_ARG(p, "%s: null params", who);
+  BSA_CHECK_ARG(p->q && p->o && ((p->k_cache && p->v_cache) || p->num_pages == 0), "%s: null tensor pointer", who);
+  BSA_CHECK_ARG(p->crow && p->col, "%s: null layout pointer", who);
+  BSA_CHECK_ARG((p->block_tables || p->max_pages == 0) && p->seqlens, "%s: null block table or lengths", who);
+  BSA_CHECK_ARG(p->batch >= 0 && p->hq >= 1 && p->hkv >= 1 && p->d >= 1 && p->total_q >= 0 && p->max_pages >= 0 &&
+                    p->page_size >= 1 && p->num_pages >= 0,
+                "%s: bad shape batch=%d hq=%d hkv=%d d=%d total_q=%d max_pages=%d page_size=%d num_pages=%d", who,
+                p->batch, p->hq, p->hkv, p->d, p->total_q, p->max_pages, p->page_size, p->num_pages);
+  BSA_CHECK_ARG(p->hq % p->hkv == 0, "%s: hq=%d is not a multiple of hkv=%d", who, p->hq, p->hkv);
+  BSA_CHECK_ARG(p->h_pat == 1 || p->h_pat == p->hkv || p->h_pat == p->hq,
+                "%s: pattern has %d heads, expected 1, %d or %d", who, p->h_pat, p->hkv, p->hq);
+  const int bs = p->block_size;
+  BSA_CHECK_ARG(bs >= 16 && bs <= 128 && (bs & (bs - 1)) == 0,
+                "%s: block_size must be a power of two in [16,128], got %d", who, bs);
+  BSA_CHECK_ARG(known_dtype(p->dtype), "%s: unknown dtype %d", who, p->dtype);
+  BSA_CHECK_ARG(p->kv_dtype == p->dtype || (p->kv_dtype == BSA_F8E4M3 && p->dtype != BSA_F32),
+                "%s: the cache has q's type, or is e4m3 under f16/bf16 queries", who);
+  BSA_CHECK_ARG(p->cu_q || p->total_q == p->batch, "%s: without cu_q there is one query token per request", who);
+  return BSA_OK;
+}
+
+template <typename T>
+int launch_rows(const bsa_paged_params* p, cudaStream_t s) {
+  const int64_t rows = (int64_t)p->total_q * p->hq, grid = (rows + 7) / 8;
+  if (grid > 0x7fffffffLL) {
+    set_error("bsa_paged_fwd: too many rows for one launch");
+    return BSA_E_TOOBIG;
+  }
+  if (p->kv_dtype == BSA_F8E4M3) {
+    if constexpr (sizeof(T) == 2) paged_rows_kernel<T, uint8_t><<<(unsigned)grid, 256, 0, s>>>(*p);
+  } else {
+    paged_rows_kernel<T, T><<<(unsigned)grid, 256, 0, s>>>(*p);
+  }
+  return check_launch("paged_rows_kernel");
+}
+
+template <typename T, typename C>
+int launch_write(const bsa_paged_write_params* p, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int kOut = V * sizeof(C);      // bytes that a thread stores
+  const int64_t in[] = {p->k_st, p->k_sh, p->v_st, p->v_sh};
+  const int64_t out[] = {p->kc_sp, p->kc_ss, p->kc_sh, p->vc_sp, p->vc_ss, p->vc_sh};
+  bool wide = p->d % V == 0 && reinterpret_cast<uintptr_t>(p->k) % 16 == 0 && reinterpret_cast<uintptr_t>(p->v) % 16 == 0 &&
+              reinterpret_cast<uintptr_t>(p->k_cache) % kOut == 0 && reinterpret_cast<uintptr_t>(p->v_cache) % kOut == 0;
+  for (int64_t x : in) wide = wide && x % V == 0;
+  for (int64_t x : out) wide = wide && x % V == 0;
+  const int64_t total = (int64_t)p->tokens * p->hkv * (p->d / (wide ? V : 1));
+  const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 8 * 4);
+  if (wide) paged_write_kernel<T, C, V><<<dim3(grid, 2), 256, 0, s>>>(*p);
+  else paged_write_kernel<T, C, 1><<<dim3(grid, 2), 256, 0, s>>>(*p);
+  return check_launch("paged_write_kernel");
+}
+}  // namespace
+}  // namespace bsa
+
+using namespace bsa;
+
+extern "C" {
+
+int bsa_paged_step(const bsa_paged_step_params* p, void* stream) {
+  BSA_CHECK_ARG(p, "bsa_paged_step: null params");
+  BSA_CHECK_ARG(p->cu_seqlen_q && p->num_free && p->short_pages, "bsa_paged_step: null pointer");
+  BSA_CHECK_ARG(p->batch >= 0 && p->max_pages >= 0 && p->free_capacity >= 0 && p->page_size >= 1 && p->max_tokens >= 0,
+                "bsa_paged_step: bad shape batch=%d max_pages=%d free_capacity=%d page_size=%d max_tokens=%d", p->batch,
+                p->max_pages, p->free_capacity, p->page_size, p->max_tokens);
+  BSA_CHECK_ARG(p->batch == 0 || (p->block_tables && p->page_counts && p->context_lens && p->new_lens && p->seqlens),
+                "bsa_paged_step: null pointer");
+  BSA_CHECK_ARG((p->free_capacity == 0 || p->free_pages) && (p->max_tokens == 0 || (p->slots && p->positions)),
+                "bsa_paged_step: null pointer");
+  if (p->batch > BSA_PAGED_STEP_MAX_BATCH || (int64_t)p->batch * p->max_pages > 0x7fffffffLL) {
+    set_error("bsa_paged_step: %d requests of %d pages; at most %d requests and 2^31 table entries", p->batch, p->max_pages,
+              BSA_PAGED_STEP_MAX_BATCH);
+    return BSA_E_TOOBIG;
+  }
+  const size_t smem = (size_t)(4 * p->batch + 1) * sizeof(int);
+  BSA_CHECK_CUDA(cudaFuncSetAttribute(paged_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const int ctas = (int64_t)p->max_tokens + 16 * (int64_t)p->batch > 4 * kStepThreads ? 8 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kStepThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  BSA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_step_kernel, *p, ctas));
+  return check_launch("paged_step_kernel");
+}
+
+int bsa_paged_write(const bsa_paged_write_params* p, void* stream) {
+  BSA_CHECK_ARG(p, "bsa_paged_write: null params");
+  BSA_CHECK_ARG(p->tokens >= 0 && p->hkv >= 1 && p->d >= 1 && p->page_size >= 1 && p->num_pages >= 0,
+                "bsa_paged_write: bad shape tokens=%d hkv=%d d=%d page_size=%d num_pages=%d", p->tokens, p->hkv, p->d,
+                p->page_size, p->num_pages);
+  BSA_CHECK_ARG(known_dtype(p->dtype), "bsa_paged_write: unknown dtype %d", p->dtype);
+  BSA_CHECK_ARG(p->cache_dtype == p->dtype || p->cache_dtype == BSA_F8E4M3,
+                "bsa_paged_write: the cache has k's type or is e4m3");
+  BSA_CHECK_ARG(p->cache_dtype != BSA_F8E4M3 || (p->k_scale > 0.f && p->v_scale > 0.f),
+                "bsa_paged_write: an e4m3 cache needs positive scales");
+  if (p->tokens == 0 || p->num_pages == 0) return BSA_OK;
+  BSA_CHECK_ARG(p->k && p->v && p->k_cache && p->v_cache && p->slots, "bsa_paged_write: null pointer");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f8 = p->cache_dtype == BSA_F8E4M3;
+  switch (p->dtype) {
+    case BSA_F16: return f8 ? launch_write<__half, uint8_t>(p, s) : launch_write<__half, __half>(p, s);
+    case BSA_BF16: return f8 ? launch_write<__nv_bfloat16, uint8_t>(p, s) : launch_write<__nv_bfloat16, __nv_bfloat16>(p, s);
+    default: return f8 ? launch_write<float, uint8_t>(p, s) : launch_write<float, float>(p, s);
+  }
+}
+
+int bsa_paged_commit(const bsa_paged_commit_params* p, void* stream) {
+  BSA_CHECK_ARG(p, "bsa_paged_commit: null params");
+  BSA_CHECK_ARG(p->batch >= 0 && p->hkv >= 1 && p->d >= 1 && p->total_q >= 0 && p->max_pages >= 0 && p->page_size >= 1 &&
+                    p->num_pages >= 0,
+                "bsa_paged_commit: bad shape batch=%d hkv=%d d=%d total_q=%d max_pages=%d page_size=%d num_pages=%d",
+                p->batch, p->hkv, p->d, p->total_q, p->max_pages, p->page_size, p->num_pages);
+  BSA_CHECK_ARG(known_dtype(p->cache_dtype) || p->cache_dtype == BSA_F8E4M3, "bsa_paged_commit: unknown dtype %d",
+                p->cache_dtype);
+  if (p->batch == 0) return BSA_OK;
+  BSA_CHECK_ARG(((p->k_cache && p->v_cache) || p->num_pages == 0) && (p->block_tables || p->max_pages == 0) && p->context_lens && p->cu_q && p->accepted &&
+                    p->new_context_lens, "bsa_paged_commit: null pointer");
+  if (p->batch > 65535) {
+    set_error("bsa_paged_commit: at most 65535 requests");
+    return BSA_E_TOOBIG;
+  }
+  const int eb = p->cache_dtype == BSA_F8E4M3 ? 1 : (int)dtype_size(p->cache_dtype);
+  const int64_t strides[] = {p->kc_sp, p->kc_ss, p->kc_sh, p->vc_sp, p->vc_ss, p->vc_sh};
+  bool wide = p->d * eb % 16 == 0 && reinterpret_cast<uintptr_t>(p->k_cache) % 16 == 0 &&
+              reinterpret_cast<uintptr_t>(p->v_cache) % 16 == 0;
+  for (int64_t x : strides) wide = wide && x * eb % 16 == 0;
+  const int vb = wide ? 16 : eb;
+  const int64_t pieces = (int64_t)2 * p->hkv * (p->d * eb / vb);
+  const dim3 grid((unsigned)std::min<int64_t>((pieces + 255) / 256, 64), p->batch);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (wide) paged_commit_kernel<uint4><<<grid, 256, 0, s>>>(*p, eb);
+  else if (eb == 4) paged_commit_kernel<uint32_t><<<grid, 256, 0, s>>>(*p, eb);
+  else if (eb == 2) paged_commit_kernel<uint16_t><<<grid, 256, 0, s>>>(*p, eb);
+  else paged_commit_kernel<uint8_t><<<grid, 256, 0, s>>>(*p, eb);
+  return check_launch("paged_commit_kernel");
+}
+
+size_t bsa_paged_workspace_bytes(const bsa_paged_params* p) {
+  if (validate_paged(p, "bsa_paged_workspace_bytes")) return 0;
+  return 0;
+}
+
+const char* bsa_paged_why_not_sm100(const bsa_paged_params* p) {
+  if (validate_paged(p, "bsa_paged_why_not_sm100")) return last_error();
+  return "no tensor-core kernel yet";
+}
+
+int bsa_paged_fwd(const bsa_paged_params* p, void* stream) {
+  int rc = validate_paged(p, "bsa_paged_fwd");
+  if (rc) return rc;
+  if (p->batch == 0 || p->total_q == 0) return BSA_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->impl == BSA_IMPL_SM100) {
+    set_error("bsa_paged_fwd: the tcgen05 kernel does not serve this call: %s", bsa_paged_why_not_sm100(p));
+    return BSA_E_UNSUPPORTED;
+  }
+  if (p->d > 256) {
+    set_error("bsa_paged_fwd: head dim %d is above 256", p->d);
+    return BSA_E_UNSUPPORTED;
+  }
+  switch (p->dtype) {
+    case BSA_F16: return launch_rows<__half>(p, s);
+    case BSA_BF16: return launch_rows<__nv_bfloat16>(p, s);
+    default: return launch_rows<float>(p, s);
+  }
+}
+
+}  // extern "C"

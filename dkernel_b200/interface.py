@@ -150,16 +150,32 @@ class SparseAttention(torch.nn.Module):
                 return_lse: bool = False,
                 split_qkv: Optional[callable] = None,
                 kv_scales: Optional[Tuple[float, float]] = None,
+                block_tables: Optional[Tensor] = None,
+                tree_mask: Optional[Tensor] = None,
                 ) -> Tensor:
         """As the reference's forward.  One extension (its README lists it as future work): a decode
         call (one query token per sequence) may pass ``k`` and ``v`` as ``torch.float8_e4m3fn``
         tensors together with ``kv_scales = (k_scale, v_scale)``; they stand for ``k * k_scale``
-        and ``v * v_scale``, and the kernel reads half the bytes."""
+        and ``v * v_scale``, and the kernel reads half the bytes.
+
+        Another: with ``block_tables`` (batch, pages per request) int32, ``k`` and ``v`` are paged caches,
+        (pages, page size, kv heads, dim), or (pages, kv heads, page size, dim) for ``seq_dim=2``, in q's
+        type or e4m3, and q is packed (tokens, heads, dim).  ``seqlens`` (batch,) counts the stored tokens
+        of each request, its query tokens' own included (see :func:`dkernel_b200.write_paged_kv`);
+        ``cu_seqlen_q`` (batch + 1,) says whose the query tokens are (None: one each).  The last tokens of a
+        request are its queries: a chain, or with ``tree_mask`` a tree of at most 64 drafted tokens, where
+        bit j of the 64-bit word ``tree_mask[t]`` says that query t attends draft j of its request (its
+        ancestors and itself).  A draft's position, which picks its pattern row and column, is the
+        context's length plus the number of other drafts it attends.  Causal modules only; no gradients.
+        Rows that attend nothing are 0 with LSE -inf; rows of ``out`` behind the last request stay as they
+        are.  The LSE is (heads, tokens)."""
         inf_kwargs = {"cu_seqlen_k": cu_seqlen_k,
                       "cu_seqlen_q": cu_seqlen_q,
                       "left_paddings": left_paddings,
                       "seqlens": seqlens,
-                      "kv_scales": kv_scales}
+                      "kv_scales": kv_scales,
+                      "block_tables": block_tables,
+                      "tree_mask": tree_mask}
         kwargs = {**self.kwargs, "return_lse": return_lse, "split_qkv": split_qkv, "_plan": self._plan()}
         buf = self._buffers
         output, lse = _sparse_attention.apply(

@@ -657,6 +657,108 @@ def _backward(ctx, do: Tensor, dlse: Optional[Tensor], dq=None, dk=None, dv=None
     return dq, dk, dv
 
 
+def _index32(t: Tensor, shape: Tuple[int, ...], device_index: int, name: str) -> Tensor:
+    """An index tensor as the kernels read it: int32, contiguous, on the call's device."""
+    assert t.shape == shape, f"{name} has shape {tuple(t.shape)}, expected {shape}"
+    if t.dtype != torch.int32 or t.get_device() != device_index:
+        assert t.is_cuda and t.get_device() == device_index, f"{name} is on {t.device}, q is on cuda:{device_index}"
+        assert t.dtype in (torch.int64, torch.int32), f"{name} must be int32, got {t.dtype}"
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _paged_cache(k_cache: Tensor, v_cache: Tensor, seq_dim: int) -> Tuple[int, int, int, int, Tuple[int, ...]]:
+    """(pages, page size, kv heads, dim, page / slot / head strides of K, then V) of a paged cache."""
+    shape = k_cache.shape
+    assert len(shape) == 4 and v_cache.shape == shape, \
+        f"paged caches are 4-D and alike, got {tuple(shape)} and {tuple(v_cache.shape)}"
+    assert k_cache.dtype == v_cache.dtype, f"cache dtypes differ: {k_cache.dtype}, {v_cache.dtype}"
+    ks, vs = k_cache.stride(), v_cache.stride()
+    assert (ks[3] == 1 and vs[3] == 1) or shape[3] == 1, "the head dim of a paged cache must be contiguous"
+    s, h = seq_dim, 3 - seq_dim
+    return shape[0], shape[s], shape[h], shape[3], (ks[0], ks[s], ks[h], vs[0], vs[s], vs[h])
+
+
+def _block_tables(t: Tensor, batch: int, device_index: int) -> Tensor:
+    assert t.dim() == 2 and t.size(0) == batch, f"block_tables has shape {tuple(t.shape)}, expected ({batch}, pages)"
+    assert t.dtype == torch.int32 and t.get_device() == device_index and (t.stride(1) == 1 or t.size(1) <= 1), \
+        f"block_tables must be int32 with contiguous rows on the call's device, got {t.dtype} on {t.device}"
+    return t
+
+
+def _tree_mask(t: Optional[Tensor], tokens: int, device_index: int) -> Optional[Tensor]:
+    if t is None:
+        return None
+    assert t.shape == (tokens,) and t.dtype == torch.int64 and t.get_device() == device_index, \
+        (f"tree_mask must be int64 ({tokens},) on the call's device (one 64-bit word per drafted token), "
+         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, inf_kwargs):
+    """Packed query tokens over a paged K/V cache (no counterpart in the reference)."""
+    assert causal, "a paged cache is only served by causal modules"
+    assert q.dim() == 3, f"queries over a paged cache are packed (tokens, heads, dim), got {tuple(q.shape)}"
+    for name in ("cu_seqlen_k", "left_paddings"):
+        assert inf_kwargs.get(name, None) is None, f"{name} does not apply to a paged cache"
+    dev = q.get_device()
+    T, hq, d = q.shape
+    pages, page_size, hkv, dk, strides = _paged_cache(k, v, seq_dim)
+    assert dk == d and hq % hkv == 0, f"q is {tuple(q.shape)}, the cache has {hkv} heads of {dk}"
+    n_pat = plan.crow.size(0)
+    assert n_pat in (1, hkv, hq), f"q and the cache have ({hq}, {hkv}) heads, the sparse pattern has {n_pat}"
+    seqlens = inf_kwargs.get("seqlens", None)
+    assert seqlens is not None and seqlens.dim() == 1, "a paged cache needs seqlens, the stored tokens of each request"
+    batch = seqlens.size(0)
+    seqlens = _index32(seqlens, (batch,), dev, "seqlens")
+    cu_q = inf_kwargs.get("cu_seqlen_q", None)
+    if cu_q is None:
+        assert T == batch, f"without cu_seqlen_q there is one query token per request, got {T} for {batch}"
+    else:
+        cu_q = _index32(cu_q, (batch + 1,), dev, "cu_seqlen_q")
+    tables = _block_tables(inf_kwargs["block_tables"], batch, dev)
+    mask = _tree_mask(inf_kwargs.get("tree_mask", None), T, dev)
+    fp8 = _fp8_kv_scales(q, k, inf_kwargs.get("kv_scales"))
+    k_scale, v_scale = fp8 if fp8 is not None else (1.0, 1.0)
+    sm_scale = sm_scale or 1. / math.sqrt(float(d))
+    # strides and alignment that TMA takes; a head past the next token's would make the tensor map's strides descend
+    q = _tma_friendly(q)
+    if q.stride(0) < q.stride(1):
+        q = q.contiguous()
+    if out is None:
+        o = _empty_like(q)
+    else:
+        o = out
+        assert o.shape == q.shape and o.dtype == q.dtype and o.get_device() == dev and (d == 1 or o.stride(2) == 1), \
+            "out must have q's shape, dtype and device and a contiguous head dim"
+    lse = torch.full((hq, T), float("-inf"), dtype=torch.float32, device=q.device) if return_lse else None
+    if T == 0 or batch == 0:
+        return o, lse
+    own = plan
+    if plan.block_size == 128 and impl != _lib.IMPL_GENERIC:
+        plan = plan.for_kernels(q)         # the same attention in blocks of 64
+    q_st, q_sh, _ = q.stride()
+    o_st, o_sh, _ = o.stride()
+    crow_sh, col_sh, h_pat, n_rows, block_size = plan.layout_dims()
+    p = _lib.PagedParams.from_buffer_copy(_lib.PAGED_PACK.pack(
+        q.data_ptr(), o.data_ptr(), _lib.ptr(lse), q_st, q_sh, o_st, o_sh, T,
+        k.data_ptr(), v.data_ptr(), *strides, tables.data_ptr(), tables.stride(0),
+        seqlens.data_ptr(), _lib.ptr(cu_q), _lib.ptr(mask), plan.crow.data_ptr(),
+        plan.col.data_ptr() or plan.crow.data_ptr(),          # a pattern without blocks has no columns
+        crow_sh, col_sh, h_pat, n_rows, block_size, 1 if own.heads_shared_in_group(hq, hkv) else 0,
+        batch, hq, hkv, d, T, tables.size(1), page_size, pages,
+        _lib.dtype_code(q.dtype), _lib.BSA_F8E4M3 if fp8 is not None else _lib.dtype_code(q.dtype),
+        float(sm_scale), k_scale, v_scale, impl, 0))
+    lib = _lib.lib()
+    need = lib.bsa_paged_workspace_bytes(C.byref(p))
+    ws = None
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        p.ws = ws.data_ptr()
+    _lib.launch(lib.bsa_paged_fwd, p, dev, "bsa_paged_fwd")
+    return o, lse
+
+
 # --------------------------------------------------------------------------- autograd
 class _sparse_attention(torch.autograd.Function):
 
@@ -687,6 +789,14 @@ class _sparse_attention(torch.autograd.Function):
                                               else None)]
 
         qs, ks = q.shape, k.shape
+        if inf_kwargs.get("block_tables", None) is not None:
+            ctx.support_backward = False
+            ctx.message = "attention over a paged cache has no backward"
+            output, lse = _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, inf_kwargs)
+            if lse is not None:
+                ctx.mark_non_differentiable(lse)
+            return output, lse
+        assert inf_kwargs.get("tree_mask", None) is None, "tree_mask needs a paged cache (block_tables)"
         hdim = 3 - (seq_dim or 1) if len(qs) == 4 else 1
         n_pat = layout_csr[0].shape[0]
         assert n_pat == 1 or n_pat == ks[hdim] or n_pat == qs[hdim], \

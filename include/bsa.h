@@ -353,6 +353,120 @@ size_t bsa_xchg_buffer_bytes(int32_t world, int64_t rows, int32_t d);
 int bsa_xchg_merge(const bsa_xchg_params* p, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged K/V cache.  No counterpart in the reference, whose caches are
+ * contiguous.  Pages of `page_size` token slots; logical token s of request b
+ * lies in slot s % page_size of page block_tables[b][s / page_size].  K and V
+ * have the same page numbers and strides of their own.  A page number outside
+ * [0, num_pages), or a logical page past the table's width, stands for tokens
+ * that do not exist: they are neither written, moved nor attended.
+ * ------------------------------------------------------------------------- */
+
+/* One step's bookkeeping: every request b grows by new_lens[b] tokens behind
+ * its context_lens[b] and holds exactly ceil((context + new) / page_size) pages
+ * afterwards (at most max_pages).  Surplus pages of all requests are pushed on
+ * the stack free_pages[0 .. num_free) in the order (request, page), then the
+ * missing ones are popped from its top in that order; where the stack runs
+ * empty the table gets -1 and *short_pages counts the pages that were missing.
+ * A request with no context and no new tokens gives back all it holds.
+ * block_tables, page_counts, free_pages and num_free are updated in place.
+ * Negative lengths count as 0; new tokens past max_tokens in all are dropped. */
+typedef struct {
+  int32_t* block_tables;      /* (batch, max_pages), rows table_stride elements apart   */
+  int64_t table_stride;
+  int32_t* page_counts;       /* (batch,) pages that each request holds                 */
+  int32_t* free_pages;        /* (free_capacity,) stack                                 */
+  int32_t* num_free;          /* (1,)                                                   */
+  const int32_t* context_lens;
+  const int32_t* new_lens;
+  const int64_t* tree_mask;   /* (max_tokens,) as in bsa_paged_params, or NULL          */
+  int32_t* cu_seqlen_q;       /* out (batch + 1,)                                       */
+  int32_t* seqlens;           /* out (batch,) context + new                             */
+  int64_t* slots;             /* out (max_tokens,) page * page_size + slot, -1 = none   */
+  int32_t* positions;         /* out (max_tokens,) context + drafts attended; 0 behind the last request */
+  int32_t* short_pages;       /* out (1,)                                               */
+  int32_t batch;              /* at most BSA_PAGED_STEP_MAX_BATCH                       */
+  int32_t max_pages, free_capacity, page_size, max_tokens;
+} bsa_paged_step_params;
+
+#define BSA_PAGED_STEP_MAX_BATCH 8192
+
+int bsa_paged_step(const bsa_paged_step_params* p, void* stream);
+
+/* cache[slots[t]] = k[t], v[t] for every token t with a slot in [0, num_pages *
+ * page_size).  With cache_dtype = BSA_F8E4M3 the stored byte is k / k_scale
+ * rounded to nearest even and saturated at +-448 (NaN stays NaN).  Slots are
+ * distinct; of two tokens with one slot either may stay. */
+typedef struct {
+  const void* k; const void* v;         /* (tokens, hkv, d)                             */
+  int64_t k_st, k_sh, v_st, v_sh;       /* token / head strides                         */
+  void* k_cache; void* v_cache;
+  int64_t kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh;   /* page / slot / head strides     */
+  const int64_t* slots;                 /* (tokens,)                                    */
+  int32_t tokens, hkv, d, page_size, num_pages;
+  int32_t dtype, cache_dtype;
+  float k_scale, v_scale;
+} bsa_paged_write_params;
+
+int bsa_paged_write(const bsa_paged_write_params* p, void* stream);
+
+/* Block-sparse attention over the pages for the drafted tokens of every request
+ * (trees, chains, single tokens).  Request b has n = cu_q[b+1] - cu_q[b] query
+ * tokens; their keys are stored, too: seqlens[b] tokens in all, the first
+ * L = seqlens[b] - n its context, draft j at logical token L + j.  With
+ * tree_mask, bit j of tree_mask[cu_q[b] + i] says that query i attends draft j
+ * (its ancestors and itself; only drafts 0..63 can be named); without, j <= i.
+ * The position of draft i is L + the number of other drafts it attends.  Query i
+ * of head h attends
+ *   context token s           iff the pattern has block (pos_i / bs, s / bs),
+ *   draft j that its mask has iff the pattern has block (pos_i / bs, pos_j / bs).
+ * A row that attends nothing: o = 0, lse = -inf.  Rows of q behind cu_q[batch]
+ * are left alone.  Every query that an entry does not attend is independent of
+ * it, whatever the entry's keys and values hold (infinities and NaN included). */
+typedef struct {
+  const void* q; void* o; float* lse;   /* (total_q, hq, d) x 2, (hq, total_q) or NULL  */
+  int64_t q_st, q_sh, o_st, o_sh, lse_sh;
+  const void* k_cache; const void* v_cache;
+  int64_t kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh;
+  const int32_t* block_tables; int64_t table_stride;
+  const int32_t* seqlens;               /* (batch,)                                     */
+  const int32_t* cu_q;                  /* (batch + 1,), NULL = one token per request   */
+  const int64_t* tree_mask;             /* (total_q,), NULL = chains                    */
+  const int32_t* crow; const int32_t* col;   /* CSR, columns ascending                  */
+  int64_t crow_sh, col_sh;
+  int32_t h_pat, n_rows, block_size;
+  int32_t heads_share;                  /* the q heads of a group have equal pattern rows */
+  int32_t batch, hq, hkv, d, total_q, max_pages, page_size, num_pages;
+  int32_t dtype, kv_dtype;              /* kv_dtype: dtype or BSA_F8E4M3                */
+  float sm_scale, k_scale, v_scale;     /* the scales apply to an e4m3 cache            */
+  int32_t impl;
+  void* ws;                             /* bsa_paged_workspace_bytes(), 256-byte aligned */
+} bsa_paged_params;
+
+size_t bsa_paged_workspace_bytes(const bsa_paged_params* p);
+int bsa_paged_fwd(const bsa_paged_params* p, void* stream);
+/* NULL if the tcgen05 kernel serves these parameters, else why not (static text). */
+const char* bsa_paged_why_not_sm100(const bsa_paged_params* p);
+
+/* The accepted branch of every request's drafts becomes part of its context:
+ * the branch of draft a = accepted[b] is the drafts that a attends and a itself
+ * (without tree_mask drafts 0..a), in the order of their numbers; its r-th one
+ * moves from logical token L + j to L + r in both caches, and
+ * new_context_lens[b] = L + length of the branch.  accepted[b] outside [0, n),
+ * or past 63 with tree_mask: nothing is accepted.  L = context_lens[b], n as in bsa_paged_params. */
+typedef struct {
+  void* k_cache; void* v_cache;
+  int64_t kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh;
+  const int32_t* block_tables; int64_t table_stride;
+  const int32_t* context_lens; const int32_t* cu_q; const int32_t* accepted;
+  const int64_t* tree_mask;
+  int32_t* new_context_lens;
+  int32_t batch, hkv, d, total_q, max_pages, page_size, num_pages;
+  int32_t cache_dtype;
+} bsa_paged_commit_params;
+
+int bsa_paged_commit(const bsa_paged_commit_params* p, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Device-side waits (on TMA / tensor-core completion barriers) are bounded.  A
  * wait that gives up records a non-zero code in a device status word and the
  * kernels of the library become no-ops until it is cleared.  This call

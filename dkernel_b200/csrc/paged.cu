@@ -424,13 +424,15 @@ int bsa_paged_commit(const bsa_paged_commit_params* p, void* stream) {
 }
 
 size_t bsa_paged_workspace_bytes(const bsa_paged_params* p) {
-  if (validate_paged(p, "bsa_paged_workspace_bytes")) return 0;
-  return 0;
+  const char* why = nullptr;
+  if (validate_paged(p, "bsa_paged_workspace_bytes") || p->impl == BSA_IMPL_GENERIC || !paged_sm100_supported(p, &why)) return 0;
+  return paged_sm100_workspace(p);
 }
 
 const char* bsa_paged_why_not_sm100(const bsa_paged_params* p) {
   if (validate_paged(p, "bsa_paged_why_not_sm100")) return last_error();
-  return "no tensor-core kernel yet";
+  const char* why = nullptr;
+  return paged_sm100_supported(p, &why) ? nullptr : why;
 }
 
 int bsa_paged_fwd(const bsa_paged_params* p, void* stream) {
@@ -438,9 +440,17 @@ int bsa_paged_fwd(const bsa_paged_params* p, void* stream) {
   if (rc) return rc;
   if (p->batch == 0 || p->total_q == 0) return BSA_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p->impl == BSA_IMPL_SM100) {
-    set_error("bsa_paged_fwd: the tcgen05 kernel does not serve this call: %s", bsa_paged_why_not_sm100(p));
-    return BSA_E_UNSUPPORTED;
+  if (p->impl != BSA_IMPL_GENERIC) {
+    const char* why = nullptr;
+    if (paged_sm100_supported(p, &why)) {
+      BSA_CHECK_ARG(p->ws && reinterpret_cast<uintptr_t>(p->ws) % 256 == 0,
+                    "bsa_paged_fwd: needs a workspace of bsa_paged_workspace_bytes(), 256-byte aligned");
+      return paged_sm100(p, s);
+    }
+    if (p->impl == BSA_IMPL_SM100) {
+      set_error("bsa_paged_fwd: the tcgen05 kernel does not serve this call: %s", why);
+      return BSA_E_UNSUPPORTED;
+    }
   }
   if (p->d > 256) {
     set_error("bsa_paged_fwd: head dim %d is above 256", p->d);

@@ -29,6 +29,11 @@ int make_tmap_4d(Tmap4* out, const void* base, int elem_bytes, uint64_t d, uint6
                  int64_t batch_stride_b, uint32_t box_d, uint32_t box_seq, bool swizzle128,
                  bool is_bf16);
 
+// 3-D tiled map of a packed (tokens, heads, d) tensor of a 16-bit type, 128-byte swizzled boxes of
+// box_tokens x box_heads x 64; strides in bytes, token_stride >= head_stride.
+int make_tmap_rows(CUtensorMap* out, const void* base, uint64_t d, uint64_t heads, uint64_t tokens,
+                   int64_t head_stride_b, int64_t token_stride_b, uint32_t box_heads, uint32_t box_tokens, bool is_bf16);
+
 bool tma_compatible(const void* base, int elem_bytes, int64_t ss, int64_t sh, int64_t sb);
 
 #if defined(__CUDACC__)
@@ -151,6 +156,13 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
       "%5, %6}], [%2];"
       ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
 // (d0, seq, head, batch) -> coordinates in the order the map stores them

@@ -34,6 +34,45 @@ static PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
   return fn;
 }
 
+// The encoder is a driver entry point and wants a context current on the calling thread.  A
+// thread that has not made a runtime call yet (an autograd worker entering the backward, a
+// host's worker thread) has none: binding the device's primary context once per thread costs
+// nothing afterwards.
+static void bind_context() {
+  thread_local bool context_bound = false;
+  if (!context_bound) {
+    if (cudaFree(nullptr) == cudaSuccess) context_bound = true;
+    else (void)cudaGetLastError();   // e.g. refused during stream capture: the encode decides
+  }
+}
+
+int make_tmap_rows(CUtensorMap* out, const void* base, uint64_t d, uint64_t heads, uint64_t tokens,
+                   int64_t head_stride_b, int64_t token_stride_b, uint32_t box_heads, uint32_t box_tokens, bool is_bf16) {
+  auto enc = get_encode();
+  if (!enc) {
+    set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
+    return BSA_E_CUDA;
+  }
+  bind_context();
+  // a dimension of extent 1 may have any stride: a legal one takes its place
+  const int64_t row = (int64_t)(d * 2 + 15) / 16 * 16;
+  const int64_t hs = heads > 1 ? head_stride_b : row, ts = tokens > 1 ? token_stride_b : hs * (int64_t)heads;
+  cuuint64_t gdim[3] = {d, heads, tokens};
+  cuuint64_t gstr[2] = {(cuuint64_t)hs, (cuuint64_t)ts};
+  cuuint32_t box[3] = {64, box_heads, box_tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(out, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                   const_cast<void*>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with CUresult %d (rows of %llu, %llu heads, %llu tokens, strides %lld %lld, "
+              "box %u %u)", (int)r, (unsigned long long)d, (unsigned long long)heads, (unsigned long long)tokens,
+              (long long)hs, (long long)ts, box_heads, box_tokens);
+    return BSA_E_CUDA;
+  }
+  return BSA_OK;
+}
+
 bool tma_compatible(const void* base, int elem_bytes, int64_t ss, int64_t sh, int64_t sb) {
   if (reinterpret_cast<uintptr_t>(base) % 16) return false;
   const int64_t m = 16 / elem_bytes;
@@ -49,15 +88,7 @@ int make_tmap_4d(Tmap4* out, const void* base, int elem_bytes, uint64_t d, uint6
     set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
     return BSA_E_CUDA;
   }
-  // The encoder is a driver entry point and wants a context current on the calling thread.  A
-  // thread that has not made a runtime call yet (an autograd worker entering the backward, a
-  // host's worker thread) has none: binding the device's primary context once per thread costs
-  // nothing afterwards.
-  thread_local bool context_bound = false;
-  if (!context_bound) {
-    if (cudaFree(nullptr) == cudaSuccess) context_bound = true;
-    else (void)cudaGetLastError();   // e.g. refused during stream capture: the encode below decides
-  }
+  bind_context();
   // The three outer dimensions are placed in order of increasing stride, so the
   // map looks like an ordinary padded row-major tensor whatever the caller's
   // layout ((B,S,H,D), (B,H,S,D), packed (T,H,D), views of larger tensors).

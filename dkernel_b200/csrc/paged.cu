@@ -120,76 +120,147 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(bsa_paged_step
     }
   }
 
+  // Slots and positions, four tokens of a thread at a time.  A warp's 32 tokens are consecutive: the requests of its
+  // first and last one bound the others' searches, to nothing where one request has them all.
   const int real = cu[B];
-  for (int t = rank * kStepThreads + tid; t < T; t += ctas * kStepThreads) {
-    long long slot = -1;
-    int pos = 0;
-    if (t < real) {
-      int lo = 0, hi = B;                       // cu[lo] <= t < cu[lo + 1]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cu[mid] <= t) lo = mid; else hi = mid;
-      }
-      const int b = lo, i = t - cu[b], n = cu[b + 1] - cu[b];
-      const long long ctx = max(__ldg(p.context_lens + b), 0), at = ctx + i, pi = at / P;
-      if (pi < target[b]) {
-        const int pg = pi < held[b] ? *(volatile int32_t*)(p.block_tables + (int64_t)b * p.table_stride + pi)
-                                    : popped(off[b] + (int)pi - held[b]);
-        if (pg >= 0) slot = (long long)pg * P + at % P;
-      }
-      int depth = i;
-      if (p.tree_mask) {
-        const uint64_t word = (uint64_t)__ldg(p.tree_mask + t) & low_bits(n);
-        depth = draft_depth(word, i);
-      }
-      pos = (int)min(ctx + depth, 0x7fffffffll);
+  auto request_of = [&](int t, int lo, int hi) {     // cu[b] <= t < cu[b + 1] with lo <= b < hi
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid] <= t) lo = mid; else hi = mid;
     }
-    p.slots[t] = slot;
-    p.positions[t] = pos;
+    return lo;
+  };
+  constexpr int U = 4;
+  for (int tw = (rank * (kStepThreads / 32) + warp) * (32 * U); tw < T; tw += ctas * kStepThreads * U) {
+    const int b_first = tw < real ? request_of(tw, 0, B) : 0;
+    const int b_last = tw < real ? request_of(min(tw + 32 * U, real) - 1, b_first, B) + 1 : 1;
+    long long slot[U];
+    int pos[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = tw + u * 32 + lane;
+      slot[u] = -1;
+      pos[u] = 0;
+      if (t < real) {
+        const int b = request_of(t, b_first, b_last), i = t - cu[b];
+        const long long ctx = max(__ldg(p.context_lens + b), 0), at = ctx + i;
+        // tokens past 2^31 have no page: a table holds fewer
+        const int pi = at > 0x7fffffffll ? W : (int)at / P;
+        if (pi < target[b]) {
+          const int pg = pi < held[b] ? *(volatile int32_t*)(p.block_tables + (int64_t)b * p.table_stride + pi)
+                                      : popped(off[b] + pi - held[b]);
+          if (pg >= 0) slot[u] = (long long)pg * P + ((int)at - pi * P);
+        }
+        int depth = i;
+        if (p.tree_mask) depth = draft_depth((uint64_t)__ldg(p.tree_mask + t) & low_bits(cu[b + 1] - cu[b]), i);
+        pos[u] = (int)min(ctx + depth, 0x7fffffffll);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = tw + u * 32 + lane;
+      if (t < T) {
+        p.slots[t] = slot[u];
+        p.positions[t] = pos[u];
+      }
+    }
   }
   if (ctas > 1) cluster_sync_all();   // no CTA leaves while another may still need the cluster's barrier
 }
 
 // ------------------------------------------------------------------ cache writes
-template <typename T> __device__ __forceinline__ uint8_t to_e4m3(T x, float scale) {
-  // a true division: k / scale decides ties, k * (1 / scale) would not
-  return (uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(Elem<T>::to_f(x), scale), __NV_SATFINITE, __NV_E4M3);
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery): a thread's index arithmetic costs less than its 32 bytes.
+struct FastDiv {
+  uint32_t d, m;
+  int s;
+  explicit FastDiv(uint32_t x) : d(x), s(0) {
+    while ((1ull << s) < x) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - x)) / x + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
+// x / scale, correctly rounded, from the correctly rounded reciprocal (Markstein: one residual step); where the
+// quotient is too large for the residual it is past e4m3's end anyway, and too small below its half step.  A true
+// division: k * (1 / scale) alone would decide ties the other way now and then.  (IEEE division took 92 of the 149 us
+// of 65000 tokens x 8 heads x 128.)
+__device__ __forceinline__ float quotient(float x, float scale, float rcp) {
+  const float q = x * rcp;
+  const float r = fmaf(fmaf(-q, scale, x), rcp, q);
+  return fabsf(q) < 1e30f ? r : q;
+}
+template <typename T> __device__ __forceinline__ uint16_t to_e4m3x2(T x, T y, float scale, float rcp, bool divide) {
+  float2 f;
+  f.x = Elem<T>::to_f(x);
+  f.y = Elem<T>::to_f(y);
+  if (divide) {
+    f.x = __fdiv_rn(f.x, scale);
+    f.y = __fdiv_rn(f.y, scale);
+  } else {
+    f.x = quotient(f.x, scale, rcp);
+    f.y = quotient(f.y, scale, rcp);
+  }
+  return (uint16_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
 }
 
-// Both caches in one grid: blockIdx.y = 0 for K, 1 for V.  A thread moves VEC elements (16 bytes of the input
-// where everything is aligned, else one element); consecutive threads are consecutive in (token, head, dim).
+// Both caches in one grid: blockIdx.y = 0 for K, 1 for V.  Bound by HBM: each element is read and written once.  A
+// thread moves VEC elements (16 bytes of the cache, or of the input where that is wider, if everything is aligned; else
+// one), four pieces at a time so that enough loads are in flight; consecutive threads are consecutive in (token, head, dim).
 template <typename T, typename C, int VEC>
-__global__ void __launch_bounds__(256) paged_write_kernel(bsa_paged_write_params p) {
+__global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant__ bsa_paged_write_params p, const FastDiv per_token,
+                                                          const FastDiv pieces, const FastDiv page, uint32_t total) {
+  constexpr int U = 4;
+  constexpr int kIn = VEC * (int)sizeof(T), kOut = VEC * (int)sizeof(C);
   const bool is_v = blockIdx.y != 0;
   const T* src = static_cast<const T*>(is_v ? p.v : p.k);
   C* dst = static_cast<C*>(is_v ? p.v_cache : p.k_cache);
   const int64_t st = is_v ? p.v_st : p.k_st, sh = is_v ? p.v_sh : p.k_sh;
   const int64_t cp = is_v ? p.vc_sp : p.kc_sp, cs = is_v ? p.vc_ss : p.kc_ss, ch = is_v ? p.vc_sh : p.kc_sh;
-  const float scale = is_v ? p.v_scale : p.k_scale;
-  const int pieces = p.d / VEC;
-  const int64_t per_token = (int64_t)p.hkv * pieces, total = per_token * p.tokens;
+  const float scale = is_v ? p.v_scale : p.k_scale, rcp = __frcp_rn(scale);
+  const bool divide = !(rcp >= 1.17549435e-38f && rcp < INFINITY);      // a reciprocal that is no normal number
   const int64_t slots = (int64_t)p.num_pages * p.page_size;
-  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < total; x += (int64_t)gridDim.x * 256) {
-    const int t = (int)(x / per_token), rem = (int)(x - t * per_token), h = rem / pieces, e = (rem - h * pieces) * VEC;
-    const int64_t slot = __ldg(p.slots + t);
-    if (slot < 0 || slot >= slots) continue;
-    const T* s = src + (int64_t)t * st + (int64_t)h * sh + e;
-    const int64_t page = slot / p.page_size;
-    C* o = dst + page * cp + (slot - page * p.page_size) * cs + (int64_t)h * ch + e;
-    if constexpr (VEC == 1) {
-      if constexpr (sizeof(C) == 1) *o = to_e4m3(*s, scale);
-      else *o = *s;
-    } else {
-      uint4 in = *reinterpret_cast<const uint4*>(s);
-      if constexpr (sizeof(C) == 1) {
-        const T* y = reinterpret_cast<const T*>(&in);
-        alignas(16) uint8_t out[VEC];
+  for (uint64_t x0 = (uint64_t)blockIdx.x * (256 * U) + threadIdx.x; x0 < total; x0 += (uint64_t)gridDim.x * (256 * U)) {
+    int64_t slot[U];
+    uint32_t tok[U], head[U], el[U];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) out[i] = to_e4m3(y[i], scale);
-        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(out);
-        else *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(out);
+    for (int u = 0; u < U; ++u) {
+      const uint64_t x = x0 + u * 256;
+      slot[u] = -1;
+      if (x < total) {
+        tok[u] = per_token.div((uint32_t)x);
+        const uint32_t rem = (uint32_t)x - tok[u] * per_token.d;
+        head[u] = pieces.div(rem);
+        el[u] = (rem - head[u] * pieces.d) * VEC;
+        slot[u] = __ldg(p.slots + tok[u]);
+        if (slot[u] >= slots) slot[u] = -1;
+      }
+    }
+    alignas(16) T in[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (slot[u] < 0) continue;
+      const T* s = src + (int64_t)tok[u] * st + (int64_t)head[u] * sh + el[u];
+      if constexpr (VEC == 1) in[u][0] = *s;
+      else
+#pragma unroll
+        for (int i = 0; i < kIn / 16; ++i) reinterpret_cast<uint4*>(in[u])[i] = __ldcs(reinterpret_cast<const uint4*>(s) + i);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (slot[u] < 0) continue;
+      const int64_t pg = slot[u] < 0x7fffffffll ? (int64_t)page.div((uint32_t)slot[u]) : slot[u] / p.page_size;
+      C* o = dst + pg * cp + (slot[u] - pg * p.page_size) * cs + (int64_t)head[u] * ch + el[u];
+      if constexpr (VEC == 1) {
+        if constexpr (sizeof(C) == 1) *o = (uint8_t)to_e4m3x2<T>(in[u][0], in[u][0], scale, rcp, divide);
+        else *o = in[u][0];
+      } else if constexpr (sizeof(C) == 1) {
+        alignas(16) uint16_t out[VEC / 2];
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) out[i] = to_e4m3x2<T>(in[u][2 * i], in[u][2 * i + 1], scale, rcp, divide);
+        *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(out);
       } else {
-        *reinterpret_cast<uint4*>(o) = in;
+#pragma unroll
+        for (int i = 0; i < kOut / 16; ++i) reinterpret_cast<uint4*>(o)[i] = reinterpret_cast<const uint4*>(in[u])[i];
       }
     }
   }
@@ -315,21 +386,29 @@ int launch_rows(const bsa_paged_params* p, cudaStream_t s) {
   return check_launch("paged_rows_kernel");
 }
 
+template <typename T, typename C, int VEC>
+int launch_write_vec(const bsa_paged_write_params* p, cudaStream_t s) {
+  const int64_t per_token = (int64_t)p->hkv * (p->d / VEC), total = per_token * p->tokens;
+  if (total > 0x7fffffffLL) {
+    set_error("bsa_paged_write: %d tokens of %d heads x %d are too many for one call", p->tokens, p->hkv, p->d);
+    return BSA_E_TOOBIG;
+  }
+  const unsigned grid = (unsigned)std::min<int64_t>((total + 1023) / 1024, 148 * 8);
+  paged_write_kernel<T, C, VEC><<<dim3(grid, 2), 256, 0, s>>>(*p, FastDiv((uint32_t)per_token), FastDiv(p->d / VEC),
+                                                               FastDiv(p->page_size), (uint32_t)total);
+  return check_launch("paged_write_kernel");
+}
+
 template <typename T, typename C>
 int launch_write(const bsa_paged_write_params* p, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T);
-  constexpr int kOut = V * sizeof(C);      // bytes that a thread stores
+  constexpr int V = 16 / sizeof(C);      // 16 bytes stored, as many or more read
   const int64_t in[] = {p->k_st, p->k_sh, p->v_st, p->v_sh};
   const int64_t out[] = {p->kc_sp, p->kc_ss, p->kc_sh, p->vc_sp, p->vc_ss, p->vc_sh};
   bool wide = p->d % V == 0 && reinterpret_cast<uintptr_t>(p->k) % 16 == 0 && reinterpret_cast<uintptr_t>(p->v) % 16 == 0 &&
-              reinterpret_cast<uintptr_t>(p->k_cache) % kOut == 0 && reinterpret_cast<uintptr_t>(p->v_cache) % kOut == 0;
-  for (int64_t x : in) wide = wide && x % V == 0;
+              reinterpret_cast<uintptr_t>(p->k_cache) % 16 == 0 && reinterpret_cast<uintptr_t>(p->v_cache) % 16 == 0;
+  for (int64_t x : in) wide = wide && x * (int64_t)sizeof(T) % 16 == 0;
   for (int64_t x : out) wide = wide && x % V == 0;
-  const int64_t total = (int64_t)p->tokens * p->hkv * (p->d / (wide ? V : 1));
-  const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 8 * 4);
-  if (wide) paged_write_kernel<T, C, V><<<dim3(grid, 2), 256, 0, s>>>(*p);
-  else paged_write_kernel<T, C, 1><<<dim3(grid, 2), 256, 0, s>>>(*p);
-  return check_launch("paged_write_kernel");
+  return wide ? launch_write_vec<T, C, V>(p, s) : launch_write_vec<T, C, 1>(p, s);
 }
 }  // namespace
 }  // namespace bsa

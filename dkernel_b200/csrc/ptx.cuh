@@ -175,6 +175,20 @@ __device__ __forceinline__ void tma_load_tile(void* dst, const Tmap4* tm, uint64
   const int c3 = tm->seq_pos == 3 ? s : (tm->head_pos == 3 ? h : b);
   tma_load_4d(dst, &tm->map, bar, d0, c1, c2, c3);
 }
+// The same with an L2 eviction policy (createpolicy).
+__device__ __forceinline__ void tma_load_tile_hint(void* dst, const Tmap4* tm, uint64_t* bar, int d0, int s, int h, int b,
+                                                   uint64_t policy) {
+  if (tm->head_bcast) h = 0;
+  if (tm->batch_bcast) b = 0;
+  const int c1 = tm->seq_pos == 1 ? s : (tm->head_pos == 1 ? h : b);
+  const int c2 = tm->seq_pos == 2 ? s : (tm->head_pos == 2 ? h : b);
+  const int c3 = tm->seq_pos == 3 ? s : (tm->head_pos == 3 ? h : b);
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2], %7;" ::"r"(smem_u32(dst)),
+      "l"(&tm->map), "r"(smem_u32(bar)), "r"(d0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
+      : "memory");
+}
 // untiled bulk copy global -> shared (both addresses 16-byte aligned, bytes a multiple of 16)
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(

@@ -19,7 +19,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .ops import _Plan, _sparse_attention
+from .ops import _Plan, _paged_forward, _sparse_attention
 from .utils import (dense_to_ccol_row, dense_to_crow_col, get_sparse_attn_mask, is_kv_cache_efficient,
                     merge_split_fwd_kernel_blocks, multiple_of, verify_sparse_pattern, zero_stride)
 
@@ -169,6 +169,11 @@ class SparseAttention(torch.nn.Module):
         context's length plus the number of other drafts it attends.  Causal modules only; no gradients.
         Rows that attend nothing are 0 with LSE -inf; rows of ``out`` behind the last request stay as they
         are.  The LSE is (heads, tokens)."""
+        if block_tables is not None and k is not None and v is not None and not (
+                torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+            # serving: nothing for autograd to record
+            return _paged_forward(self._plan(), self.kwargs, self.seq_dim, q, k, v, sm_scale, block_tables, seqlens,
+                                  cu_seqlen_q, tree_mask, kv_scales, return_lse, cu_seqlen_k, left_paddings)
         inf_kwargs = {"cu_seqlen_k": cu_seqlen_k,
                       "cu_seqlen_q": cu_seqlen_q,
                       "left_paddings": left_paddings,

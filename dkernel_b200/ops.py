@@ -695,30 +695,36 @@ def _tree_mask(t: Optional[Tensor], tokens: int, device_index: int) -> Optional[
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, inf_kwargs):
+def _paged_forward(plan, kwargs, seq_dim, q, k, v, sm_scale, block_tables, seqlens, cu_q, tree_mask, kv_scales, return_lse,
+                   cu_seqlen_k, left_paddings):
+    """Paged attention as ``SparseAttention.forward`` calls it when no gradient can be asked for."""
+    _check_inputs(q, k, v)
+    assert cu_seqlen_k is None and left_paddings is None, "cu_seqlen_k and left_paddings do not apply to a paged cache"
+    o, lse = _paged(q, k, v, sm_scale, plan, 1 if seq_dim is None else seq_dim, kwargs["causal"], kwargs.get("out"),
+                    _IMPL_NAMES[kwargs.get("impl")], return_lse, block_tables, seqlens, cu_q, tree_mask, kv_scales)
+    return (o, lse) if return_lse else o
+
+
+def _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, tables, seqlens, cu_q, mask, kv_scales):
     """Packed query tokens over a paged K/V cache (no counterpart in the reference)."""
     assert causal, "a paged cache is only served by causal modules"
     assert q.dim() == 3, f"queries over a paged cache are packed (tokens, heads, dim), got {tuple(q.shape)}"
-    for name in ("cu_seqlen_k", "left_paddings"):
-        assert inf_kwargs.get(name, None) is None, f"{name} does not apply to a paged cache"
     dev = q.get_device()
     T, hq, d = q.shape
     pages, page_size, hkv, dk, strides = _paged_cache(k, v, seq_dim)
     assert dk == d and hq % hkv == 0, f"q is {tuple(q.shape)}, the cache has {hkv} heads of {dk}"
     n_pat = plan.crow.size(0)
     assert n_pat in (1, hkv, hq), f"q and the cache have ({hq}, {hkv}) heads, the sparse pattern has {n_pat}"
-    seqlens = inf_kwargs.get("seqlens", None)
     assert seqlens is not None and seqlens.dim() == 1, "a paged cache needs seqlens, the stored tokens of each request"
     batch = seqlens.size(0)
     seqlens = _index32(seqlens, (batch,), dev, "seqlens")
-    cu_q = inf_kwargs.get("cu_seqlen_q", None)
     if cu_q is None:
         assert T == batch, f"without cu_seqlen_q there is one query token per request, got {T} for {batch}"
     else:
         cu_q = _index32(cu_q, (batch + 1,), dev, "cu_seqlen_q")
-    tables = _block_tables(inf_kwargs["block_tables"], batch, dev)
-    mask = _tree_mask(inf_kwargs.get("tree_mask", None), T, dev)
-    fp8 = _fp8_kv_scales(q, k, inf_kwargs.get("kv_scales"))
+    tables = _block_tables(tables, batch, dev)
+    mask = _tree_mask(mask, T, dev)
+    fp8 = _fp8_kv_scales(q, k, kv_scales)
     k_scale, v_scale = fp8 if fp8 is not None else (1.0, 1.0)
     sm_scale = sm_scale or 1. / math.sqrt(float(d))
     # strides and alignment that TMA takes; a head past the next token's would make the tensor map's strides descend
@@ -792,7 +798,11 @@ class _sparse_attention(torch.autograd.Function):
         if inf_kwargs.get("block_tables", None) is not None:
             ctx.support_backward = False
             ctx.message = "attention over a paged cache has no backward"
-            output, lse = _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, inf_kwargs)
+            for name in ("cu_seqlen_k", "left_paddings"):
+                assert inf_kwargs.get(name, None) is None, f"{name} does not apply to a paged cache"
+            output, lse = _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, inf_kwargs["block_tables"],
+                                 inf_kwargs["seqlens"], inf_kwargs["cu_seqlen_q"], inf_kwargs["tree_mask"],
+                                 inf_kwargs["kv_scales"])
             if lse is not None:
                 ctx.mark_non_differentiable(lse)
             return output, lse

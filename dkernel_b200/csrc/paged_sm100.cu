@@ -62,6 +62,7 @@ struct PPlanHead {
 struct PPlan : PPlanHead {
   uint32_t tb[32];             // by pattern row: which of the blocks r0, r0 + 1, ... it has
   uint64_t dm[8];              // drafts whose position lies in block r0 + y
+  uint32_t special[2];         // listed blocks that hold drafts, miss a page, or are not attended by every pattern row
   uint32_t col[kSeg], fl[kSeg];
   int page[kSegPages];
 };
@@ -328,6 +329,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     int e = tl->start_e;
     const int per_entry = sh.box == BS ? 1 : BS / sh.box;      // pages of a block
     const int most = min(kSeg, kSegPages / per_entry), batch = min(most, 32);
+    const uint32_t all_pages = (1u << per_entry) - 1u;
     long long base = tl->start_base;
     // the loads' own ring: the 16-bit tiles, or the e4m3 tiles that the converters read
     constexpr int NL = KV8 ? NR : NS;
@@ -449,6 +451,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           pl = &tl->plan[pb];
           pl->tb[lane] = my_tb;
           if (lane < 8) pl->dm[lane] = my_dm;
+          if (lane < 2) pl->special[lane] = 0u;
           if (lane == 0) {
             pl->valid = 1;
             pl->first = first;
@@ -459,6 +462,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           first = false;
           n = 0;
+          __syncwarp();
         };
         auto publish = [&](bool last) {
           const int nt = (n + E - 1) / E;
@@ -510,9 +514,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         };
         open();
         if (!ok) break;
+        bool windows = nf > 1;
+        // flags of a block that all rows attend (those that there are: heads of the last piece, rows of the pattern)
+        const uint32_t all_rows = windows ? __ballot_sync(0xffffffffu, lane < nf && fg < gcnt) : 1u;
         const int ny = owns_tail ? (ik.Sp - 1) / BS - r0 + 1 : 0;
         int clo = 0, chi = 0, wc = 0, wi = kWindow;
-        bool windows = nf > 1;
         if (windows) {
           // several rows: the union of their columns inside the share's range, a window of columns at a time
           clo = ia == 0 ? 0 : __ldg(cols0 + beg0 + ia);
@@ -594,9 +600,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               pl->page[at * per_entry + z] = pg;
               have |= (pg >= 0 ? 1u : 0u) << z;
             }
-            if (per_entry == 1) have = 0u - have & 0xffu;      // a block that lies in one page
             pl->col[at] = (uint32_t)col | have << 23 | tail;
             pl->fl[at] = fl;
+            if (tail || have != all_pages || fl != all_rows) atomicOr(&pl->special[at >> 5], 1u << (at & 31));
           }
           n += cnt;
         }
@@ -773,6 +779,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (lane == 0) mbar_arrive(&tl->q_ready);
         }
       }
+      // blocks past the last one of a tile that is not full are as special as any
+      const uint64_t special = dry ? 0ull : ((uint64_t)pl->special[1] << 32 | pl->special[0]) | ~low_bits(n);
       // ---- one K/V tile; this repetition weighs CW of its 64 keys
       auto softmax_tile = [&](auto cw, uint64_t M, uint32_t tSb) -> bool {
         constexpr int CW = decltype(cw)::value;
@@ -878,43 +886,43 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int j = 0; j < nt; ++j, gs += dry ? 0 : 1) {
         const int sb = gs & 1, s = gs % NS;
         // ---- which of the tile's 64 keys this row attends, before the logits are there
-        uint64_t M = 0;
+        uint64_t M = ~0ull;
         int clear0 = 64;                      // rows of V that hold no key of this item, from here to the end of their block
-        bool clear = false;
-#pragma unroll
-        for (int en = 0; en < E; ++en) {
-          const int idx = j * E + en;
-          if (idx < n) {
-            const uint32_t c = pl->col[idx];
+        bool clear = false, any_att = warp_live;
+        if ((special >> (j * E)) & low_bits(E)) {
+          M = 0;
+#pragma unroll 1
+          for (int en = 0; en < E; ++en) {
+            const int idx = j * E + en;
             uint64_t me = 0;
-            if (!(c & kTailFlag)) {
-              if ((pl->fl[idx] >> f) & 1u) me = low_bits(BS);
-            } else {
-              const int y = (int)(c & kColMask) - pl->r0, s0 = (int)(c & kColMask) * BS;
-              const int nc = min(max(pl->Lp - s0, 0), BS);           // context tokens of the block
-              if (nc && (tbits & 1u)) me = low_bits(nc);             // only block r0 holds any
-              if (tree) {
-                const int d0 = s0 + nc - pl->L;                      // first draft of the block
-                if (d0 < 64) me |= (fm >> d0) << nc;
-              } else if (y < 32 && ((tbits >> y) & 1u)) {
-                me |= low_bits(min(max(pos - s0 + 1, 0), BS));
+            if (idx < n) {
+              const uint32_t c = pl->col[idx];
+              if (!(c & kTailFlag)) {
+                if ((pl->fl[idx] >> f) & 1u) me = low_bits(BS);
+              } else {
+                const int y = (int)(c & kColMask) - pl->r0, s0 = (int)(c & kColMask) * BS;
+                const int nc = min(max(pl->Lp - s0, 0), BS);           // context tokens of the block
+                if (nc && (tbits & 1u)) me = low_bits(nc);             // only block r0 holds any
+                if (tree) {
+                  const int d0 = s0 + nc - pl->L;                      // first draft of the block
+                  if (d0 < 64) me |= (fm >> d0) << nc;
+                } else if (y < 32 && ((tbits >> y) & 1u)) {
+                  me |= low_bits(min(max(pos - s0 + 1, 0), BS));
+                }
+                me &= low_bits(BS);
+                const int len = pl->Sp - s0;
+                if (len < BS) { clear = true; clear0 = en * BS + len; }
               }
-              me &= low_bits(BS);
-              const int len = pl->Sp - s0;
-              if (len < BS) { clear = true; clear0 = en * BS + len; }
-            }
-            const uint32_t have = (c >> 23) & 0xffu;
-            if (me && have != 0xffu) {
-              if (sh.box == BS) me = 0;
-              else
+              const uint32_t have = (c >> 23) & 0xffu;
+              if (me && have != low_bits(BS / sh.box))
                 for (int i = 0; i < BS / sh.box; ++i)
                   if (!((have >> i) & 1u)) me &= ~(low_bits(sh.box) << (i * sh.box));
             }
             M |= me << (en * BS);
           }
+          any_att = __any_sync(0xffffffffu, row_ok && M != 0ull);
+          if (!row_ok) M = ~0ull;             // nobody reads these rows: nothing to mask
         }
-        const bool any_att = __any_sync(0xffffffffu, row_ok && M != 0ull);
-        if (!row_ok) M = ~0ull;               // nobody reads these rows: nothing to mask
         if (!dry && !mbar_wait(&tl->qk_done[sb], (gs >> 1) & 1, wait_status, 1032)) { alive = false; break; }
         tc_fence_after();
         if (clear) {

@@ -44,16 +44,77 @@ __device__ __forceinline__ long long block_scan(long long x, long long* warp_sum
   return x;
 }
 
+// Slots and positions of the step's tokens, by the warp `w` of `warps`, U tokens of a lane at a time.  The 32 * U tokens of
+// a warp are consecutive: the requests of its first and last one bound the others' searches, to nothing where one request
+// has them all.  page(b, i): page i of request b.
+constexpr int kStepTokens = 4096;      // up to so many the tables' kernel does them itself
+template <typename F>
+__device__ __forceinline__ void step_tokens(const bsa_paged_step_params& p, const int* cu, int w, int warps, int lane, F page) {
+  constexpr int U = 4;
+  const int B = p.batch, P = p.page_size, T = p.max_tokens, real = cu[B];
+  auto request_of = [&](int t, int lo, int hi) {     // cu[b] <= t < cu[b + 1] with lo <= b < hi
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid] <= t) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
+  const int per = T <= 32 * warps ? 1 : U;           // few tokens: spread over the warps
+  for (int tw = w * (32 * per); tw < T; tw += warps * (32 * per)) {
+    const int b_first = tw < real ? request_of(tw, 0, B) : 0;
+    const int b_last = tw < real ? request_of(min(tw + 32 * per, real) - 1, b_first, B) + 1 : 1;
+    long long slot[U];
+    int pos[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = tw + u * 32 + lane;
+      slot[u] = -1;
+      pos[u] = 0;
+      if (u < per && t < real) {
+        const int b = request_of(t, b_first, b_last), i = t - cu[b];
+        const long long ctx = max(__ldg(p.context_lens + b), 0), at = ctx + i;
+        // tokens past 2^31 have no page: a table holds fewer
+        const int pi = at > 0x7fffffffll ? 0x7fffffff : (int)at / P, pg = page(b, pi);
+        if (pg >= 0) slot[u] = (long long)pg * P + ((int)at - pi * P);
+        int depth = i;
+        if (p.tree_mask) depth = draft_depth((uint64_t)__ldg(p.tree_mask + t) & low_bits(cu[b + 1] - cu[b]), i);
+        pos[u] = (int)min(ctx + depth, 0x7fffffffll);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = tw + u * 32 + lane;
+      if (u < per && t < T) {
+        p.slots[t] = slot[u];
+        p.positions[t] = pos[u];
+      }
+    }
+  }
+}
+
+// The same for many tokens, over the whole machine, from the finished tables.
+__global__ void __launch_bounds__(256) paged_slots_kernel(const bsa_paged_step_params p) {
+  extern __shared__ int slots_smem[];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int b = threadIdx.x; b <= p.batch; b += 256) slots_smem[b] = p.cu_seqlen_q[b];
+  __syncthreads();
+  step_tokens(p, slots_smem, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8, threadIdx.x & 31, [&](int b, int pi) {
+    return pi < p.page_counts[b] ? p.block_tables[(int64_t)b * p.table_stride + pi] : -1;
+  });
+}
+
 __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(bsa_paged_step_params p, int ctas) {
   extern __shared__ int step_smem[];
   __shared__ long long warp_sums[32];
-  const int B = p.batch, P = p.page_size, T = p.max_tokens, W = p.max_pages;
+  const int B = p.batch, P = p.page_size, W = p.max_pages;
+  const int T = p.max_tokens;
   int* cu = step_smem;            // [B + 1]
   int* held = cu + B + 1;         // [B] pages before the step
   int* target = held + B;         // [B] pages after it
   int* off = target + B;          // [B] first push (target < held) or first pop
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int n_free = min(max(__ldg(p.num_free), 0), p.free_capacity);
   long long new_before = 0, moved_before = 0;
@@ -120,51 +181,12 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(bsa_paged_step
     }
   }
 
-  // Slots and positions, four tokens of a thread at a time.  A warp's 32 tokens are consecutive: the requests of its
-  // first and last one bound the others' searches, to nothing where one request has them all.
-  const int real = cu[B];
-  auto request_of = [&](int t, int lo, int hi) {     // cu[b] <= t < cu[b + 1] with lo <= b < hi
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cu[mid] <= t) lo = mid; else hi = mid;
-    }
-    return lo;
-  };
-  constexpr int U = 4;
-  for (int tw = (rank * (kStepThreads / 32) + warp) * (32 * U); tw < T; tw += ctas * kStepThreads * U) {
-    const int b_first = tw < real ? request_of(tw, 0, B) : 0;
-    const int b_last = tw < real ? request_of(min(tw + 32 * U, real) - 1, b_first, B) + 1 : 1;
-    long long slot[U];
-    int pos[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = tw + u * 32 + lane;
-      slot[u] = -1;
-      pos[u] = 0;
-      if (t < real) {
-        const int b = request_of(t, b_first, b_last), i = t - cu[b];
-        const long long ctx = max(__ldg(p.context_lens + b), 0), at = ctx + i;
-        // tokens past 2^31 have no page: a table holds fewer
-        const int pi = at > 0x7fffffffll ? W : (int)at / P;
-        if (pi < target[b]) {
-          const int pg = pi < held[b] ? *(volatile int32_t*)(p.block_tables + (int64_t)b * p.table_stride + pi)
-                                      : popped(off[b] + pi - held[b]);
-          if (pg >= 0) slot[u] = (long long)pg * P + ((int)at - pi * P);
-        }
-        int depth = i;
-        if (p.tree_mask) depth = draft_depth((uint64_t)__ldg(p.tree_mask + t) & low_bits(cu[b + 1] - cu[b]), i);
-        pos[u] = (int)min(ctx + depth, 0x7fffffffll);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = tw + u * 32 + lane;
-      if (t < T) {
-        p.slots[t] = slot[u];
-        p.positions[t] = pos[u];
-      }
-    }
-  }
+  if (p.max_tokens <= kStepTokens)
+    step_tokens(p, cu, rank * (kStepThreads / 32) + warp, ctas * (kStepThreads / 32), lane, [&](int b, int pi) {
+      if (pi >= target[b]) return -1;
+      return pi < held[b] ? *(volatile int32_t*)(p.block_tables + (int64_t)b * p.table_stride + pi)
+                          : popped(off[b] + pi - held[b]);
+    });
   if (ctas > 1) cluster_sync_all();   // no CTA leaves while another may still need the cluster's barrier
 }
 
@@ -205,12 +227,13 @@ template <typename T> __device__ __forceinline__ uint16_t to_e4m3x2(T x, T y, fl
 
 // Both caches in one grid: blockIdx.y = 0 for K, 1 for V.  Bound by HBM: each element is read and written once.  A
 // thread moves VEC elements (16 bytes of the cache, or of the input where that is wider, if everything is aligned; else
-// one), four pieces at a time so that enough loads are in flight; consecutive threads are consecutive in (token, head, dim).
+// one), 64 bytes at a time so that enough loads are in flight; consecutive threads are consecutive in (token, head, dim).
+// (Four CTAs per SM: with 124 registers, two, 65000 tokens x 8 heads x 128 into e4m3 took 119 us.)
 template <typename T, typename C, int VEC>
-__global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant__ bsa_paged_write_params p, const FastDiv per_token,
+__global__ void __launch_bounds__(256, 4) paged_write_kernel(const __grid_constant__ bsa_paged_write_params p, const FastDiv per_token,
                                                           const FastDiv pieces, const FastDiv page, uint32_t total) {
-  constexpr int U = 4;
   constexpr int kIn = VEC * (int)sizeof(T), kOut = VEC * (int)sizeof(C);
+  constexpr int U = kIn > 16 ? 2 : 4;
   const bool is_v = blockIdx.y != 0;
   const T* src = static_cast<const T*>(is_v ? p.v : p.k);
   C* dst = static_cast<C*>(is_v ? p.v_cache : p.k_cache);
@@ -393,7 +416,8 @@ int launch_write_vec(const bsa_paged_write_params* p, cudaStream_t s) {
     set_error("bsa_paged_write: %d tokens of %d heads x %d are too many for one call", p->tokens, p->hkv, p->d);
     return BSA_E_TOOBIG;
   }
-  const unsigned grid = (unsigned)std::min<int64_t>((total + 1023) / 1024, 148 * 8);
+  const int64_t per_cta = 256 * (VEC * sizeof(T) > 16 ? 2 : 4);
+  const unsigned grid = (unsigned)std::min<int64_t>((total + per_cta - 1) / per_cta, 148 * 16);
   paged_write_kernel<T, C, VEC><<<dim3(grid, 2), 256, 0, s>>>(*p, FastDiv((uint32_t)per_token), FastDiv(p->d / VEC),
                                                                FastDiv(p->page_size), (uint32_t)total);
   return check_launch("paged_write_kernel");
@@ -434,7 +458,7 @@ int bsa_paged_step(const bsa_paged_step_params* p, void* stream) {
   }
   const size_t smem = (size_t)(4 * p->batch + 1) * sizeof(int);
   BSA_CHECK_CUDA(cudaFuncSetAttribute(paged_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  const int ctas = (int64_t)p->max_tokens + 16 * (int64_t)p->batch > 4 * kStepThreads ? 8 : 1;
+  const int ctas = p->max_tokens + 16 * (int64_t)p->batch > 4 * kStepThreads ? 8 : 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kStepThreads);
@@ -447,7 +471,14 @@ int bsa_paged_step(const bsa_paged_step_params* p, void* stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   BSA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_step_kernel, *p, ctas));
-  return check_launch("paged_step_kernel");
+  if (p->max_tokens <= kStepTokens) return check_launch("paged_step_kernel");
+  cfg.gridDim = dim3((unsigned)std::min(296, cdiv_i(p->max_tokens, 1024)));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = (size_t)(p->batch + 1) * sizeof(int);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  BSA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_slots_kernel, *p));
+  return check_launch("paged_slots_kernel");
 }
 
 int bsa_paged_write(const bsa_paged_write_params* p, void* stream) {

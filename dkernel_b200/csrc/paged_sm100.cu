@@ -71,18 +71,19 @@ template <int D, bool KV8> struct PGeo {
   static constexpr int kSub = D / 64;
   static constexpr int kQTile = 128 * D * 2;
   static constexpr int kTile = 64 * D * 2;
-  // 16-bit K slots and V slots.  An e4m3 cache needs one of each (two at D = 64): K's is free again when Q K^T is done
-  static constexpr int kSlots = (D == 64 ? 4 : 2) / (KV8 ? 2 : 1);
+  // 16-bit K and V slots.  With an e4m3 cache K's is free again when Q K^T is done, V's only behind the softmax: V has two
+  static constexpr int kKSlots = KV8 ? (D == 64 ? 2 : 1) : (D == 64 ? 4 : 2);
+  static constexpr int kVSlots = D == 64 && !KV8 ? 4 : 2;
   static constexpr int kRawTile = 64 * D;
-  static constexpr int kRaw = KV8 ? (D == 64 ? 4 : 2) : 1;                     // e4m3 K slots, and V slots
+  static constexpr int kRaw = KV8 ? (D == 64 ? 4 : 1) : 1;                     // e4m3 K slots, and V slots
   static constexpr int kRawBytes = KV8 ? 2 * kRaw * kRawTile : 0;
-  static constexpr size_t kFixed = 1024 + kQTile + 2 * kSlots * kTile + kRawBytes;
+  static constexpr size_t kFixed = 1024 + kQTile + (kKSlots + kVSlots) * kTile + kRawBytes;
   static constexpr int kThreads = KV8 ? 256 : 192;
 };
 
-template <int NS, int NR> struct PTail {
+template <int NK, int NV, int NR> struct PTail {
   uint64_t plan_full[2], plan_free[2], q_full, q_free;
-  uint64_t k_full[NS], v_full[NS], k_free[NS], v_free[NS];
+  uint64_t k_full[NK], v_full[NV], k_free[NK], v_free[NV];
   uint64_t raw_k_full[NR], raw_v_full[NR], raw_k_free[NR], raw_v_free[NR];
   uint64_t qk_done[2], p_full[2], pv_done[2], o_free, met, q_ready;
   uint32_t tmem_base;
@@ -198,32 +199,31 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   // converted row by row with a power of two of their own (their largest value comes to 2^13 .. 2^14; what f16 then
   // cannot hold is below 2^-38 of that), which the row's logits are divided by again.
   constexpr bool BE = BF16 && !KV8, QCONV = BF16 && KV8;
-  constexpr int kSub = Geo::kSub, NS = Geo::kSlots, NR = Geo::kRaw, kTile = Geo::kTile, kThreads = Geo::kThreads;
+  constexpr int kSub = Geo::kSub, NK = Geo::kKSlots, NV = Geo::kVSlots, NR = Geo::kRaw, kTile = Geo::kTile, kThreads = Geo::kThreads;
   constexpr int E = 64 / BS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + Geo::kQTile;
-  uint8_t* sV = sK + NS * kTile;
-  uint8_t* sRawK = sV + NS * kTile;
+  uint8_t* sV = sK + NK * kTile;
+  uint8_t* sRawK = sV + NV * kTile;
   uint8_t* sRawV = sRawK + NR * Geo::kRawTile;
-  auto* tl = reinterpret_cast<PTail<NS, NR>*>(sV + NS * kTile + Geo::kRawBytes);
+  auto* tl = reinterpret_cast<PTail<NK, NV, NR>*>(sV + NV * kTile + Geo::kRawBytes);
 
   // the joining kernel reads nothing before this grid has ended; its launch may be prepared
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (*reinterpret_cast<volatile int*>(wait_status) != 0) return;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int cta = blockIdx.x;
+  const int warp = tid >> 5;
 
   if (tid == 0) {
     constexpr int kFollow = KV8 ? 7 : 5;       // issuer, four softmax warps (and two converters)
     for (int i = 0; i < 2; ++i) { mbar_init(&tl->plan_full[i], 1); mbar_init(&tl->plan_free[i], kFollow); }
     mbar_init(&tl->q_full, 1);
     mbar_init(&tl->q_free, 1);
-    for (int i = 0; i < NS; ++i) {
-      mbar_init(&tl->k_full[i], KV8 ? 2 : 1); mbar_init(&tl->v_full[i], KV8 ? 2 : 1);
-      mbar_init(&tl->k_free[i], 1); mbar_init(&tl->v_free[i], 1);
-    }
+    for (int i = 0; i < NK; ++i) { mbar_init(&tl->k_full[i], KV8 ? 2 : 1); mbar_init(&tl->k_free[i], 1); }
+    for (int i = 0; i < NV; ++i) { mbar_init(&tl->v_full[i], KV8 ? 2 : 1); mbar_init(&tl->v_free[i], 1); }
     for (int i = 0; i < NR; ++i) {
       mbar_init(&tl->raw_k_full[i], 1); mbar_init(&tl->raw_v_full[i], 1);
       mbar_init(&tl->raw_k_free[i], 2); mbar_init(&tl->raw_v_free[i], 2);
@@ -332,7 +332,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t all_pages = (1u << per_entry) - 1u;
     long long base = tl->start_base;
     // the loads' own ring: the 16-bit tiles, or the e4m3 tiles that the converters read
-    constexpr int NL = KV8 ? NR : NS;
+    constexpr int NLK = KV8 ? NR : NK, NLV = KV8 ? NR : NV;
     constexpr uint32_t kLoadBytes = KV8 ? Geo::kRawTile : kTile;
     uint64_t* kf = KV8 ? tl->raw_k_full : tl->k_full;
     uint64_t* vf = KV8 ? tl->raw_v_full : tl->v_full;
@@ -475,9 +475,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const bool is_v = t == 2 * nt - 1 || (t > 0 && !(t & 1));
             const int j = t == 2 * nt - 1 ? nt - 1 : is_v ? t / 2 - 1 : (t + 1) / 2;
             const uint32_t x = rg + (uint32_t)j;
-            const int s = x % NL;
+            const int s = is_v ? x % NLV : x % NLK;
             uint64_t* full = (is_v ? vf : kf) + s;
-            if (!mbar_wait((is_v ? ve : ke) + s, ((x / NL) & 1) ^ 1, wait_status, is_v ? 1014 : 1013)) { ok = false; break; }
+            if (!mbar_wait((is_v ? ve : ke) + s, ((is_v ? x / NLV : x / NLK) & 1) ^ 1, wait_status, is_v ? 1014 : 1013)) { ok = false; break; }
             if (lane == 0) mbar_expect_tx(full, kLoadBytes);
             __syncwarp();
             if (lane < per * subs) {
@@ -641,8 +641,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       auto qk = [&](int j) -> bool {
         const uint32_t x = g + (uint32_t)j;
-        const int s = x % NS, sb = x & 1;
-        if (!mbar_wait(&tl->k_full[s], (x / NS) & 1, wait_status, 1023)) return false;
+        const int s = x % NK, sb = x & 1;
+        if (!mbar_wait(&tl->k_full[s], (x / NK) & 1, wait_status, 1023)) return false;
         tc_fence_after();
         const uint64_t kd = kdesc + (uint64_t)((s * kTile) >> 4);
         if (elect_one()) {
@@ -660,8 +660,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int j = 0; ok && j < nt && j < 2; ++j) ok = qk(j);
       for (int j = 0; ok && j < nt; ++j) {
         const uint32_t x = g + (uint32_t)j;
-        const int s = x % NS, sb = x & 1;
-        if (!mbar_wait(&tl->v_full[s], (x / NS) & 1, wait_status, 1024)) { ok = false; break; }
+        const int s = x % NV, sb = x & 1;
+        if (!mbar_wait(&tl->v_full[s], (x / NV) & 1, wait_status, 1024)) { ok = false; break; }
         if (!mbar_wait(&tl->p_full[sb], (x >> 1) & 1, wait_status, 1025)) { ok = false; break; }
         // the item before has read O
         if (!started && items > 1 && !mbar_wait(&tl->o_free, (items - 2) & 1, wait_status, 1026)) { ok = false; break; }
@@ -884,7 +884,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         return true;
       };
       for (int j = 0; j < nt; ++j, gs += dry ? 0 : 1) {
-        const int sb = gs & 1, s = gs % NS;
+        const int sb = gs & 1, s = gs % NV;
         // ---- which of the tile's 64 keys this row attends, before the logits are there
         uint64_t M = ~0ull;
         int clear0 = 64;                      // rows of V that hold no key of this item, from here to the end of their block
@@ -927,9 +927,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tc_fence_after();
         if (clear) {
           // keys behind the item's end: P is 0 there, and 0 times whatever the page holds has to be 0, too
-          // (with one V slot its barrier may still be in the phase of the tile before, whose product then has to be over)
-          if (NS == 1 && gs > 0 && !mbar_wait(&tl->pv_done[(gs - 1) & 1], ((gs - 1) >> 1) & 1, wait_status, 1037)) { alive = false; break; }
-          if (!mbar_wait(&tl->v_full[s], (gs / NS) & 1, wait_status, 1033)) { alive = false; break; }
+          // (two V slots at least: this tile's barrier cannot still be in the phase of the tile before in its slot, whose
+          // product was over before this tile's logits were there)
+          if (!mbar_wait(&tl->v_full[s], (gs / NV) & 1, wait_status, 1033)) { alive = false; break; }
           uint8_t* vt = sV + s * kTile;
           const int cend = (clear0 / BS + 1) * BS;
           for (int q = r; q < (cend - clear0) * kSub * 8; q += 128) {
@@ -1151,12 +1151,21 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const PPlan* pl = &tl->plan[pb];
       if (pl->valid < 0) break;
       const int nt = pl->nt;
-      auto convert = [&](int j, const uint8_t* raw, uint8_t* tile, uint64_t* rf, uint64_t* re, uint64_t* full, uint64_t* empty,
-                         int code) -> bool {
+      bool ok = true;
+      // in the order of the loads: K a tile ahead of V
+      for (int t = 0; ok && t < 2 * nt; ++t) {
+        const bool is_v = t == 2 * nt - 1 || (t > 0 && !(t & 1));
+        const int j = t == 2 * nt - 1 ? nt - 1 : is_v ? t / 2 - 1 : (t + 1) / 2;
         const uint32_t x = rg + (uint32_t)j;
-        const int rs = x % NR, s = x % NS;
-        if (!mbar_wait(&rf[rs], (x / NR) & 1, wait_status, code)) return false;
-        if (!mbar_wait(&empty[s], ((x / NS) & 1) ^ 1, wait_status, code + 1)) return false;
+        const int rs = x % NR, s = is_v ? x % NV : x % NK;
+        const uint8_t* raw = is_v ? sRawV : sRawK;
+        uint8_t* tile = is_v ? sV : sK;
+        uint64_t* full = is_v ? tl->v_full : tl->k_full;
+        uint64_t* empty = is_v ? tl->v_free : tl->k_free;
+        uint64_t* rf = is_v ? tl->raw_v_full : tl->raw_k_full;
+        uint64_t* re = is_v ? tl->raw_v_free : tl->raw_k_free;
+        if (!mbar_wait(&rf[rs], (x / NR) & 1, wait_status, is_v ? 1044 : 1042)) { ok = false; break; }
+        if (!mbar_wait(&empty[s], ((is_v ? x / NV : x / NK) & 1) ^ 1, wait_status, is_v ? 1045 : 1043)) { ok = false; break; }
         const uint8_t* src = raw + rs * Geo::kRawTile;
         uint8_t* dst = tile + s * kTile;
         // 16 values a lane and turn, the two warps in turns.  A lane keeps its place in the row, and its rows are 8 apart, so
@@ -1166,19 +1175,26 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint8_t* from = src + ((warp - kWConv) * 32 + lane) * 16;
         uint8_t* base = dst + odd * 8192 + row * 128;
         const int a0 = ((c0 + odd) ^ (row & 7)) * 16, a1 = ((c0 + 1 - odd) ^ (row & 7)) * 16;
-#pragma unroll 8
-        for (int q = 0; q < 32 / kRows; ++q) {
-          const uint4 v = *reinterpret_cast<const uint4*>(from + q * 1024);
-          const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-          uint32_t out[8];
+        // Turns go four at a time, their loads before any store: the compiler cannot tell the tiles apart and would wait
+        // for each turn's load (1000 cycles a tile of 64 x 128)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            out[2 * i] = e4m3x2_to_f16((uint16_t)in[i]);
-            out[2 * i + 1] = e4m3x2_to_f16((uint16_t)(in[i] >> 16));
+        for (int q0 = 0; q0 < 32 / kRows; q0 += 4) {
+          uint4 v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const uint4*>(from + (q0 + q) * 1024);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t in[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+            uint32_t out[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              out[2 * i] = e4m3x2_to_f16((uint16_t)in[i]);
+              out[2 * i + 1] = e4m3x2_to_f16((uint16_t)(in[i] >> 16));
+            }
+            const uint4 lo = make_uint4(out[0], out[1], out[2], out[3]), hi = make_uint4(out[4], out[5], out[6], out[7]);
+            *reinterpret_cast<uint4*>(base + (q0 + q) * 2 * kRows * 128 + a0) = odd ? hi : lo;
+            *reinterpret_cast<uint4*>(base + (q0 + q) * 2 * kRows * 128 + a1) = odd ? lo : hi;
           }
-          const uint4 lo = make_uint4(out[0], out[1], out[2], out[3]), hi = make_uint4(out[4], out[5], out[6], out[7]);
-          *reinterpret_cast<uint4*>(base + q * 2 * kRows * 128 + a0) = odd ? hi : lo;
-          *reinterpret_cast<uint4*>(base + q * 2 * kRows * 128 + a1) = odd ? lo : hi;
         }
         fence_proxy_async();
         __syncwarp();
@@ -1186,13 +1202,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           mbar_arrive(&full[s]);
           mbar_arrive(&re[rs]);
         }
-        return true;
-      };
-      bool ok = true;
-      if (nt > 0) ok = convert(0, sRawK, sK, tl->raw_k_full, tl->raw_k_free, tl->k_full, tl->k_free, 1042);
-      for (int j = 0; ok && j < nt; ++j) {
-        if (j + 1 < nt) ok = convert(j + 1, sRawK, sK, tl->raw_k_full, tl->raw_k_free, tl->k_full, tl->k_free, 1042);
-        if (ok) ok = convert(j, sRawV, sV, tl->raw_v_full, tl->raw_v_free, tl->v_full, tl->v_free, 1044);
       }
       if (!ok) break;
       rg += (uint32_t)nt;
@@ -1367,7 +1376,7 @@ int launch_paged(const bsa_paged_params* p, const PagedShape& shape, cudaStream_
   auto* recs = static_cast<PagedRec*>(p->ws);
   auto* ml = reinterpret_cast<float2*>(static_cast<char*>(p->ws) + kRecBytes);
   auto* po = reinterpret_cast<float*>(static_cast<char*>(p->ws) + kRecBytes + ml_bytes(shape));
-  constexpr size_t smem = Geo::kFixed + sizeof(PTail<Geo::kSlots, Geo::kRaw>);
+  constexpr size_t smem = Geo::kFixed + sizeof(PTail<Geo::kKSlots, Geo::kVSlots, Geo::kRaw>);
   static_assert(smem <= 113 * 1024, "two CTAs per SM");
   auto kern = paged_attn_kernel<BF16, D, BS, KV8>;
   BSA_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));

@@ -29,7 +29,7 @@ constexpr int kSegPages = 128;        // and pages of theirs
 constexpr int kWindow = 128;          // columns whose union is formed at a time
 constexpr uint32_t kTailFlag = 1u << 31;
 constexpr uint32_t kColMask = (1u << 23) - 1u;   // bits 23..30: pages that exist
-constexpr int kOverhead = 2;          // an item's fixed cost in K/V tiles
+constexpr int kOverhead = 3;          // an item's fixed cost in K/V tiles
 constexpr float kRescale = 8.0f;
 constexpr int kWPlan = 4, kWIssue = 5, kWConv = 6;
 
@@ -521,8 +521,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         int clo = 0, chi = 0, wc = 0, wi = kWindow;
         if (windows) {
           // several rows: the union of their columns inside the share's range, a window of columns at a time
-          clo = ia == 0 ? 0 : __ldg(cols0 + beg0 + ia);
-          chi = owns_tail ? r0 : __ldg(cols0 + beg0 + ib);
+          // (a share's end is the next one's beginning; behind the first row's last block there is only the context's end)
+          auto border = [&](int at) { return at == 0 ? 0 : at < n0 ? __ldg(cols0 + beg0 + at) : r0; };
+          clo = border(ia);
+          chi = owns_tail ? r0 : border(ib);
           if (clo > 0) {
             int lo = cur, hi = end;
             while (lo < hi) {
@@ -1391,7 +1393,7 @@ int launch_paged(const bsa_paged_params* p, const PagedShape& shape, cudaStream_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   BSA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, tmQ, tmK, tmV, *p, sh, recs, ml, po, status));
-  cfg.gridDim = dim3(sh.ctas, cdiv_i(sh.rows_cap, 32));     // 8 warps of four rows
+  cfg.gridDim = dim3(sh.ctas, cdiv_i(sh.rows_cap, 16));     // 8 warps of four rows, or of one: twice over
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   BSA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<T16, C8, D>, *p, sh, (const PagedRec*)recs, (const float2*)ml,

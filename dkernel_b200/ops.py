@@ -73,6 +73,7 @@ class _Plan:
         self._max_head_nnz: Optional[int] = None
         self._csc_csr: Optional[Tensor] = None
         self._dims: Optional[Tuple[int, int, int, int, int]] = None
+        self._paged: Dict[Tuple, Tuple[int, ...]] = {}
 
     def layout_dims(self) -> Tuple[int, int, int, int, int]:
         """(crow head stride, col head stride, pattern heads, rows, block size) as the kernels take them."""
@@ -705,6 +706,22 @@ def _paged_forward(plan, kwargs, seq_dim, q, k, v, sm_scale, block_tables, seqle
     return (o, lse) if return_lse else o
 
 
+def _paged_statics(plan: _Plan, q: Tensor, hq: int, hkv: int, impl: int) -> Tuple[int, ...]:
+    """The layout fields of a paged call, which follow from the module and the head counts alone."""
+    key = (hq, hkv, impl, q.dtype, q.size(-1))
+    got = plan._paged.get(key)
+    if got is None:
+        n_pat = plan.crow.size(0)
+        assert n_pat in (1, hkv, hq), f"q and the cache have ({hq}, {hkv}) heads, the sparse pattern has {n_pat}"
+        kp = plan
+        if plan.block_size == 128 and impl != _lib.IMPL_GENERIC:
+            kp = plan.for_kernels(q)         # the same attention in blocks of 64
+        got = (kp.crow.data_ptr(), kp.col.data_ptr() or kp.crow.data_ptr(),     # a pattern without blocks has no columns
+               *kp.layout_dims(), 1 if plan.heads_shared_in_group(hq, hkv) else 0)
+        plan._paged[key] = got
+    return got
+
+
 def _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, tables, seqlens, cu_q, mask, kv_scales):
     """Packed query tokens over a paged K/V cache (no counterpart in the reference)."""
     assert causal, "a paged cache is only served by causal modules"
@@ -713,8 +730,6 @@ def _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, tabl
     T, hq, d = q.shape
     pages, page_size, hkv, dk, strides = _paged_cache(k, v, seq_dim)
     assert dk == d and hq % hkv == 0, f"q is {tuple(q.shape)}, the cache has {hkv} heads of {dk}"
-    n_pat = plan.crow.size(0)
-    assert n_pat in (1, hkv, hq), f"q and the cache have ({hq}, {hkv}) heads, the sparse pattern has {n_pat}"
     assert seqlens is not None and seqlens.dim() == 1, "a paged cache needs seqlens, the stored tokens of each request"
     batch = seqlens.size(0)
     seqlens = _index32(seqlens, (batch,), dev, "seqlens")
@@ -725,41 +740,37 @@ def _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, tabl
     tables = _block_tables(tables, batch, dev)
     mask = _tree_mask(mask, T, dev)
     fp8 = _fp8_kv_scales(q, k, kv_scales)
-    k_scale, v_scale = fp8 if fp8 is not None else (1.0, 1.0)
-    sm_scale = sm_scale or 1. / math.sqrt(float(d))
+    code = _lib.dtype_code(q.dtype)
+    k_scale, v_scale, kv_code = (*fp8, _lib.BSA_F8E4M3) if fp8 is not None else (1.0, 1.0, code)
+    statics = _paged_statics(plan, q, hq, hkv, impl)
     # strides and alignment that TMA takes; a head past the next token's would make the tensor map's strides descend
     q = _tma_friendly(q)
-    if q.stride(0) < q.stride(1):
+    q_st, q_sh, _ = q.stride()
+    if q_st < q_sh:
         q = q.contiguous()
+        q_st, q_sh, _ = q.stride()
     if out is None:
         o = _empty_like(q)
+        o_st, o_sh = hq * d, d
     else:
         o = out
         assert o.shape == q.shape and o.dtype == q.dtype and o.get_device() == dev and (d == 1 or o.stride(2) == 1), \
             "out must have q's shape, dtype and device and a contiguous head dim"
+        o_st, o_sh, _ = o.stride()
     lse = torch.full((hq, T), float("-inf"), dtype=torch.float32, device=q.device) if return_lse else None
     if T == 0 or batch == 0:
         return o, lse
-    own = plan
-    if plan.block_size == 128 and impl != _lib.IMPL_GENERIC:
-        plan = plan.for_kernels(q)         # the same attention in blocks of 64
-    q_st, q_sh, _ = q.stride()
-    o_st, o_sh, _ = o.stride()
-    crow_sh, col_sh, h_pat, n_rows, block_size = plan.layout_dims()
     p = _lib.PagedParams.from_buffer_copy(_lib.PAGED_PACK.pack(
         q.data_ptr(), o.data_ptr(), _lib.ptr(lse), q_st, q_sh, o_st, o_sh, T,
         k.data_ptr(), v.data_ptr(), *strides, tables.data_ptr(), tables.stride(0),
-        seqlens.data_ptr(), _lib.ptr(cu_q), _lib.ptr(mask), plan.crow.data_ptr(),
-        plan.col.data_ptr() or plan.crow.data_ptr(),          # a pattern without blocks has no columns
-        crow_sh, col_sh, h_pat, n_rows, block_size, 1 if own.heads_shared_in_group(hq, hkv) else 0,
-        batch, hq, hkv, d, T, tables.size(1), page_size, pages,
-        _lib.dtype_code(q.dtype), _lib.BSA_F8E4M3 if fp8 is not None else _lib.dtype_code(q.dtype),
-        float(sm_scale), k_scale, v_scale, impl, 0))
+        seqlens.data_ptr(), _lib.ptr(cu_q), _lib.ptr(mask), *statics,
+        batch, hq, hkv, d, T, tables.size(1), page_size, pages, code, kv_code,
+        float(sm_scale or 1. / math.sqrt(float(d))), k_scale, v_scale, impl, 0))
     lib = _lib.lib()
     need = lib.bsa_paged_workspace_bytes(C.byref(p))
     ws = None
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(need, dtype=torch.uint8)
         p.ws = ws.data_ptr()
     _lib.launch(lib.bsa_paged_fwd, p, dev, "bsa_paged_fwd")
     return o, lse

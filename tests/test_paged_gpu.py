@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import paged_oracle as P
-from paged_cases import (E4M3, check_attention, local_stride, paged_inputs, random_pattern, random_trees, words_of)
+from paged_cases import (E4M3, check_attention, local_stride, logit_error, paged_inputs, random_pattern, random_trees, words_of)
 
 pytestmark = pytest.mark.gpu
 bf16, f16, f32 = torch.bfloat16, torch.float16, torch.float32
@@ -281,6 +281,40 @@ def test_positions_past_the_pattern():
     """Rows past the pattern's last attend nothing; the request's earlier rows are served."""
     pat = local_stride(2, 4, 2, 2)
     run_case(4, 2, 64, [250, 100, 300], [12, 5, 3], 16, bf16, 64, pat, tree=False)
+
+
+def both_ways(x, pat, bs, **kw):
+    """The tensor-core kernel and the CUDA-core form of one call."""
+    single = all(n == 1 for n in x["new"])
+    got = [call(module(bs, pat, seq_dim=x["seq_dim"], impl=impl), x, single=single, return_lse=True, **kw) for impl in ("sm100", "generic")]
+    return got
+
+
+@pytest.mark.parametrize("bs,heads,fp8,tree", [(64, "q", False, True), (64, "kv", True, True), (32, "q", True, True), (16, "kv", False, False),
+                                               (64, "kv", False, False), (16, "q", False, True)])
+def test_shares_that_end_anywhere(bs, heads, fp8, tree):
+    """The items' blocks are cut into equal shares for the CTAs: batches of all sizes, rows with few blocks and without a
+    diagonal, so that cuts fall at the first, the last and no block of a row, inside and between items."""
+    hq, hkv, d, page = 4, 2, 64, 16
+    rng = random.Random(bs)
+    nb = 1024 // bs
+    for trial in range(24):
+        density = rng.choice([0.05, 0.3, 0.9])
+        pat = random_pattern({"q": hq, "kv": hkv}[heads], nb, density, trial)
+        if trial % 3 == 0:
+            pat[:, np.arange(nb), np.arange(nb)] = True
+        B = rng.randint(1, 24)
+        new = [rng.choice([1, 2, 5, rng.randint(1, 64)]) for _ in range(B)]
+        ctx = [rng.choice([0, 64, rng.randint(0, 900)]) for _ in range(B)]
+        x = paged_inputs(trial, hq, hkv, d, ctx, new, page, bf16, fp8=fp8, tree=tree)
+        (a, la), (b, lb) = both_ways(x, pat, bs)
+        # twice the bound of each against 64 bits
+        scale = 1 / math.sqrt(d)
+        e = logit_error(x, d, scale)
+        vmax = P.dequant(x["v"], (x["kv_scales"] or (1.0, 1.0))[1]).abs().max().item()
+        assert ((a - b).abs().float() <= 2 * (2.0 ** -8 * b.abs().float() * 1.01 + (4 * e + 2.0 ** -15) * vmax)).all(), (trial, B)
+        assert torch.equal(torch.isinf(la), torch.isinf(lb))
+        assert (la - lb).nan_to_num(0.0).abs().max() <= 2 * (2 * e + 2.0 ** -20 + 2.0 ** -22 * 16), (trial, B)
 
 
 def test_empty_batches():

@@ -8,9 +8,10 @@
 // and end inside an item, whose partial results a second kernel then joins.  Requests with more rows than a tile have
 // their even and odd tiles in two halves of the line of work, so that two CTAs come to the same keys at about the same
 // time and one of them finds them in L2.
-// Few rows (a token's heads, small trees) are repeated down the 128 rows of the tile, and each repetition weighs its own
-// quarter of the keys, so that all four softmax warps have a share of the exponentials; what the repetitions have
-// is added up in shared memory at the item's end.
+// Up to 16 rows (a token's heads, small trees) are repeated down the 128 rows of the tile, twice in each softmax warp's 32.
+// Each warp weighs its own quarter of the keys, so that all four have a share of the exponentials, and its second
+// repetition holds the low terms of the weights that the first holds the high terms of; what the repetitions have is added
+// up in shared memory at the item's end.
 //
 // A K/V tile is 64 tokens = 1, 2 or 4 pattern blocks, wherever their pages are: one TMA box per page piece.
 // Warps (192 threads, 256 with an e4m3 cache): 0-3 softmax and epilogue, 4 planner and TMA producer, 5 MMA issuer,
@@ -33,8 +34,8 @@ constexpr int kOverhead = 3;          // an item's fixed cost in K/V tiles
 constexpr float kRescale = 8.0f;
 constexpr int kWPlan = 4, kWIssue = 5, kWConv = 6;
 
-// How rows and items are cut; the same for the whole launch.  A tile's rows come in chunks of cr (32, 64 or 128) rows =
-// ct tokens x gt heads, what one TMA box brings.
+// How rows and items are cut; the same for the whole launch.  A tile's rows come in chunks of cr (16, 32, 64 or 128) rows
+// for ct tokens x gt heads, what one TMA box brings.
 struct PagedShape {
   int gt;          // q heads of a group that a tile holds
   int chunks;      // pieces of a group
@@ -55,7 +56,7 @@ struct PagedRec { int valid, b, t0, n, L, tok0, ntok, head0, gcnt, last; };
 struct PPlanHead {
   int valid, first, last, part;
   int n, nt;                   // listed blocks, K/V tiles
-  int rr;                      // rows of a repetition: 32, or 128 = none
+  int rr;                      // rows of a repetition: 16, or 128 = none
   int b, t0, n_new, L, kvh, head0, gcnt;
   int tok0, ntok, Lp, r0, Sp;  // Lp: keys before it are context for every row of the item; r0 = Lp / block; Sp: end of its keys
 };
@@ -242,6 +243,12 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   } else if (warp == kWIssue) {
     tmem_alloc(&tl->tmem_base, 256);
     tmem_relinquish();
+  }
+  // Rows that no box brings are zeros: products with them cost least power, and this kernel runs into the power limit
+  if (warp < 4) {
+#pragma unroll 4
+    for (int i = tid; i < Geo::kQTile / 16; i += 128) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async();
   }
   // What is above may overlap the joining kernel of the call before; what is below reads and writes memory.
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -442,7 +449,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           recs[cta] = rec;
         }
         // up to 16 rows are repeated; more would cost more at the item's end than the repetitions save at its tiles
-        const int rr = ntok * sh.gt <= 16 ? 32 : 128;
+        const int rr = sh.cr == 16 && ntok <= sh.ct ? 16 : 128;
         n = 0;
         bool first = true, begins = true;
         auto open = [&]() {
@@ -497,11 +504,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               // Q behind the first K
               if (items > 0 && !mbar_wait(&tl->q_free, (items - 1) & 1, wait_status, 1012)) { ok = false; break; }
               ++items;
-              const int pos = 128 / sh.cr, boxes = kSub * pos;      // at most 8
+              const int pos = 128 / sh.cr, boxes = kSub * pos;
               if (lane == 0) mbar_expect_tx(&tl->q_full, (uint32_t)(boxes * sh.ct * sh.gt * 128));
               __syncwarp();
               if (lane < boxes) {
-                const int at = lane & (pos - 1), c = lane / pos;
+                const int at = lane & (pos - 1), c = lane / pos;      // at most 16 boxes
                 (void)BSA_IN_BOUNDS(r.t0 + tok0 >= 0 && r.t0 + tok0 < p.total_q && head0 < p.hq, wait_status, 823);
                 tma_load_3d(sQ + c * 16384 + at * sh.cr * 128, &tmQ, &tl->q_full, c * 64, head0,
                             r.t0 + tok0 + (rr == 128 ? at : 0) * sh.ct);
@@ -636,6 +643,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const PPlan* pl = &tl->plan[pb];
       if (pl->valid < 0) break;
       const int nt = pl->nt, last = pl->last;
+      const bool split = pl->rr == 128;       // both terms of P in a row; else they have rows of their own
       if (pl->first) {
         if (!mbar_wait(QCONV ? &tl->q_ready : &tl->q_full, items & 1, wait_status, 1022)) break;
         ++items;
@@ -672,8 +680,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t acc0 = started ? 1u : 0u;
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)      // 4..7: the low terms of P
-            tc_mma_ts(tO, tS + sb * 64 + kk * 8, vd + (uint64_t)(((kk & 3) * 2048) >> 4), idesc_pv, kk ? 1u : acc0);
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_ts(tO, tS + sb * 64 + kk * 8, vd + (uint64_t)((kk * 2048) >> 4), idesc_pv, kk ? 1u : acc0);
+          if (split) {
+#pragma unroll
+            for (int kk = 4; kk < 8; ++kk)    // the low terms of P
+              tc_mma_ts(tO, tS + sb * 64 + kk * 8, vd + (uint64_t)(((kk & 3) * 2048) >> 4), idesc_pv, 1u);
+          }
           tc_commit(&tl->pv_done[sb]);
           tc_commit(&tl->v_free[s]);
         }
@@ -723,7 +736,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (pl->first) {
         const int q = r & (rr - 1), qq = q & (sh.cr - 1);
         const int tl_row = q / sh.cr * sh.ct + qq / sh.gt, g = qq % sh.gt, tok = tl_row;
-        rep = r / rr;
+        rep = warp;
         row_ok = qq < sh.ct * sh.gt && tok < pl->ntok && g < pl->gcnt;
         warp_live = __any_sync(0xffffffffu, row_ok);
         i_tok = pl->tok0 + tok;
@@ -824,7 +837,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
         }
         const bool any = __any_sync(0xffffffffu, need);
-        const bool live = att && m_used != -INFINITY;
+        const bool live = att && row_ok && m_used != -INFINITY;
         const float neg_m = kShift - m_used;
         const uint64_t scale_2 = f32x2(scale2, scale2), neg_m2 = f32x2(neg_m, neg_m);
         uint64_t sum2[2] = {0ull, 0ull};
@@ -851,17 +864,15 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             // this repetition's keys, and no weight on the others'
             uint32_t z[kHalf / 2];
 #pragma unroll
-            for (int c = 0; c < kHalf / 2; ++c) z[c] = 0u;
+            for (int c = 0; c < kHalf / 2; ++c) {
+              z[c] = 0u;
+              if (lane >= 16) pk[c] = pq[c];
+            }
 #pragma unroll
             for (int i = 0; i < 64 / CW; ++i) {
               const uint32_t at = (uint32_t)(i * (CW / 2));
-              if (i == rep) {
-                tmem_st8(tSb + at, pk);
-                tmem_st8(tSb + 32 + at, pq);
-              } else {
-                tmem_st8(tSb + at, z);
-                tmem_st8(tSb + 32 + at, z);
-              }
+              if (i == rep) tmem_st8(tSb + at, pk);
+              else tmem_st8(tSb + at, z);
             }
           }
         }
@@ -1046,11 +1057,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
         } else {
           // the repetitions' parts are weighed and added, some columns at a time, by all four warps.  Rows in use are the
-          // first nr (at most 16) of a part
+          // first nr (at most 16) of a part.  Parts: the warps' high terms, and their low terms under the same weight
           constexpr int P = 4;
           const int nr = dry ? 4 : pl->ntok * sh.gt;
-          const int q = lane;
-          if (q < nr) {
+          const int q = lane & 15;
+          if (lane < nr) {
             tl->jm[rep * nr + q] = m_used;
             tl->jl[rep * nr + q] = l;
           }
@@ -1071,7 +1082,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tl->jbad[r] = !(L >= 0.f);
           }
           int shift = D == 64 ? 6 : 7;        // 2^shift columns at a time, 16 or more: what the stage holds
-          while ((P * nr) << shift > 2048) --shift;
+          while ((2 * P * nr) << shift > 2048) --shift;
           const int cols = 1 << shift;
           bool fine = true;
           for (int c0 = 0; c0 < D; c0 += cols) {
@@ -1082,7 +1093,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               tmem_ld16(tOl + c0 + c, o);
               tmem_ld_wait();
               if (q < nr) {
-                float* dst = buf + (rep * nr + q) * cols + c;
+                float* dst = buf + ((2 * rep + (lane >> 4)) * nr + q) * cols + c;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                   reinterpret_cast<uint4*>(dst)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -1096,10 +1107,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
               for (int pp = 0; pp < P; ++pp) {
                 const float a = tl->jw[pp * nr + row];
-                const float2 v = *reinterpret_cast<const float2*>(buf + (pp * nr + row) * cols + c2);
+                const float2 v = *reinterpret_cast<const float2*>(buf + (2 * pp * nr + row) * cols + c2);
+                const float2 u = *reinterpret_cast<const float2*>(buf + ((2 * pp + 1) * nr + row) * cols + c2);
                 if (a != 0.f) {
-                  x0 = fmaf(v.x, a, x0);
-                  x1 = fmaf(v.y, a, x1);
+                  x0 = fmaf(v.x + u.x, a, x0);
+                  x1 = fmaf(v.y + u.y, a, x1);
                 }
               }
               const int tok = (int)((row + 0.5f) * sh.inv_gt), g = row - tok * sh.gt;
@@ -1330,8 +1342,9 @@ void plan_shape(const bsa_paged_params* p, PagedShape* sh) {
   }
   sh->gt = gt;
   sh->chunks = cdiv_i(G, gt);
-  sh->cr = gt <= 32 ? 32 : gt <= 64 ? 64 : 128;
-  sh->ct = sh->cr / gt;
+  // chunks of 16 rows where a tile holds no fewer tokens with them than in chunks of 32
+  sh->cr = gt <= 16 && 2 * (16 / gt) >= 32 / gt ? 16 : gt <= 32 ? 32 : gt <= 64 ? 64 : 128;
+  sh->ct = p->cu_q ? sh->cr / gt : 1;      // single tokens: the rows behind them stay zeros
   sh->tt = 128 / sh->cr * sh->ct;
   const int most = p->cu_q ? (p->total_q < sh->tt ? p->total_q : sh->tt) : 1;
   sh->rows_cap = most * gt;
@@ -1339,7 +1352,7 @@ void plan_shape(const bsa_paged_params* p, PagedShape* sh) {
   sh->inv_gt = 1.f / gt;
   // of the average request
   const int64_t mean = p->batch > 0 ? (int64_t)p->total_q / p->batch : 1;
-  sh->rr_hint = mean * gt <= 16 ? 32 : 128;
+  sh->rr_hint = sh->cr == 16 && mean <= sh->ct ? 16 : 128;
   sh->box = p->page_size < bs ? p->page_size : bs;
   sh->page_shift = 0;
   while ((1 << sh->page_shift) < p->page_size) ++sh->page_shift;

@@ -614,3 +614,201 @@ def test_speculative_decoding_end_to_end(fp8):
             for s, (kk, vv) in enumerate(story[b]):
                 pg = table[b, s // page].item()
                 assert torch.equal(kc[pg, s % page].float().cpu(), kk) and torch.equal(vc[pg, s % page].float().cpu(), vv)
+
+
+# ------------------------------------------------------------------ how it runs
+def test_which_kernel_serves():
+    """The tensor-core kernel serves every 16-bit call with its pages, blocks and strides; asked for by name it refuses the
+    others, with the reason."""
+    from dkernel_b200._lib import BsaError
+    hq, hkv, bs = 4, 2, 64
+    for d, dtype, page, fp8, why in ((128, bf16, 16, False, None), (48, f16, 8, False, None), (64, bf16, 128, True, None),
+                                     (64, f32, 16, False, "dtype"), (160, bf16, 16, False, "head dim"), (40, bf16, 16, True, "head dim"),
+                                     (64, bf16, 24, False, "page size"), (64, bf16, 4, False, "page size")):
+        x = paged_inputs(1, hq, hkv, d, [70, 3], [5, 9], page, dtype, fp8=fp8)
+        mod = module(bs, local_stride(hkv, 4, 2, 2), seq_dim=1, impl="sm100")
+        if why is None:
+            call(mod, x)
+        else:
+            with pytest.raises(BsaError, match=why):
+                call(mod, x)
+    mod = module(128, local_stride(hkv, 4, 2, 2), seq_dim=1, impl="sm100")       # refined to blocks of 64
+    call(mod, paged_inputs(1, hq, hkv, 64, [70, 3], [5, 9], 16, bf16))
+
+
+def test_same_bits_every_time():
+    x = paged_inputs(2, 8, 2, 128, [900, 333, 10], [60, 17, 1], 16, bf16)
+    mod, c = module(64, local_stride(2, 16, 3, 4), seq_dim=1), device(x)
+    first = call(mod, x, c, return_lse=True)
+    for _ in range(5):
+        again = call(mod, x, c, return_lse=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_long_cache():
+    """Pages whose offsets pass 2^32 bytes and 2^31 elements."""
+    from dkernel_b200 import commit_paged_draft, write_paged_kv
+    hkv, d, page, pages = 8, 128, 64, 40000            # 2.6e9 elements
+    kc = torch.empty((pages, page, hkv, d), dtype=bf16, device="cuda")
+    vc = torch.empty_like(kc)
+    hq, bs = 8, 64
+    g = torch.Generator().manual_seed(1)
+    T = 150
+    k, v = (torch.randn((T, hkv, d), generator=g).to(bf16) for _ in range(2))
+    used = [39999, 17, 35000]
+    slots = torch.tensor([used[t // page] * page + t % page for t in range(T)]).cuda()
+    write_paged_kv(k.cuda(), v.cuda(), kc, vc, slots)
+    assert torch.equal(kc[39999].cpu(), k[:64]) and torch.equal(vc[35000, :T - 128].cpu(), v[128:])
+    pat = local_stride(hkv, 4, 3, 2)
+    n = 10
+    q = torch.randn((n, hq, d), generator=g).to(bf16)
+    words = [P.tree_word([j - 2 if j > 1 else -1 for j in range(n)], j) for j in range(n)]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = torch.tensor([used], **i32)
+    args = dict(block_tables=table, seqlens=torch.tensor([T], **i32), cu_seqlen_q=torch.tensor([0, n], **i32),
+                tree_mask=P.as_int64(words).cuda())
+    small = torch.zeros((3, page, hkv, d), dtype=bf16)
+    small.view(-1, hkv, d)[:T] = k
+    small_v = torch.zeros_like(small)
+    small_v.view(-1, hkv, d)[:T] = v
+    ref, ref_lse, _ = P.attend(q, small, small_v, torch.tensor([[0, 1, 2]]), [T], pat, bs, cu=[0, n], words=words)
+    x = dict(q=q, k=small, v=small_v, kv_scales=None)
+    for impl in IMPLS:
+        out, lse = module(bs, pat, seq_dim=1, impl=impl)(q.cuda(), kc, vc, return_lse=True, **args)
+        check_attention(out, lse, ref, ref_lse, x, d, 1 / math.sqrt(d))
+    lens = commit_paged_draft(kc, vc, table, torch.tensor([T - n], **i32), args["cu_seqlen_q"], torch.tensor([9], **i32),
+                              tree_mask=args["tree_mask"])
+    assert lens.item() == T - n + 5
+    assert torch.equal(kc[35000, 12:17].cpu(), k[T - n + 1::2]) and torch.equal(vc[35000, 12:17].cpu(), v[T - n + 1::2])
+
+
+def test_other_streams_and_two_graphs():
+    """A step captured into two graphs (each with its workspace), replayed in turn and at the same time on two streams, with
+    new inputs in the captured buffers; an eager call on a side stream."""
+    from dkernel_b200 import commit_paged_draft, plan_paged_step, write_paged_kv
+    hq, hkv, d, bs, page, B, W = 8, 2, 128, 64, 16, 6, 40
+    pat = local_stride(hkv, 16, 3, 4)
+    mod = module(bs, pat, seq_dim=1)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    new = [9, 33, 1, 64, 17, 5]
+    T, pages = sum(new), 260
+    rng = random.Random(7)
+
+    class Server:
+        def __init__(self, seed):
+            g = torch.Generator().manual_seed(seed)
+            self.g = g
+            self.kc, self.vc = (torch.randn((pages, page, hkv, d), generator=g).to(bf16).cuda() for _ in range(2))
+            self.table, self.counts = torch.full((B, W), -1, **i32), torch.zeros(B, **i32)
+            self.free, self.top = torch.randperm(pages, generator=g).to(torch.int32).cuda(), torch.tensor([pages], **i32)
+            self.ctx, self.new = torch.zeros(B, **i32), torch.tensor(new, **i32)
+            self.q, self.k, self.v = (torch.zeros((T, h, d), dtype=bf16, device="cuda") for h in (hq, hkv, hkv))
+            self.mask, self.acc = torch.zeros(T, dtype=torch.int64, device="cuda"), torch.zeros(B, **i32)
+
+        def fill(self):
+            trees = random_trees(rng, new)
+            self.words = words_of(trees)
+            self.ctx.copy_(torch.tensor([rng.randint(0, 500) for _ in range(B)], dtype=torch.int32))
+            for t in (self.q, self.k, self.v):
+                t.copy_(torch.randn(t.shape, generator=self.g).to(bf16))
+            self.mask.copy_(P.as_int64(self.words))
+            self.acc.copy_(torch.tensor([rng.randint(-1, n - 1) for n in new], dtype=torch.int32))
+
+        def step(self):
+            st = plan_paged_step(self.table, self.counts, self.free, self.top, self.ctx, self.new, page_size=page,
+                                 max_new_tokens=T, tree_mask=self.mask)
+            write_paged_kv(self.k, self.v, self.kc, self.vc, st.slots)
+            out, lse = mod(self.q, self.kc, self.vc, block_tables=self.table, seqlens=st.seqlens, cu_seqlen_q=st.cu_seqlen_q,
+                           tree_mask=self.mask, return_lse=True)
+            lens = commit_paged_draft(self.kc, self.vc, self.table, self.ctx, st.cu_seqlen_q, self.acc, tree_mask=self.mask)
+            return out, lse, lens, st
+
+        def state(self):
+            return [t.clone() for t in (self.kc, self.vc, self.table, self.counts, self.free, self.top)]
+
+        def restore(self, s):
+            for t, x in zip((self.kc, self.vc, self.table, self.counts, self.free, self.top), s):
+                t.copy_(x)
+
+    servers, graphs, outs, streams = [Server(1), Server(2)], [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s, st in zip(servers, streams):
+        s.fill()
+        keep = s.state()
+        with torch.cuda.stream(st):
+            s.step()                                   # everything is loaded before the capture
+        torch.cuda.synchronize()
+        s.restore(keep)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            outs.append(s.step())
+        graphs.append(graph)
+    for rounds in range(4):
+        want = []
+        for s in servers:
+            s.fill()
+            keep = s.state()
+            with torch.cuda.stream(streams[0]):        # eagerly, on a side stream
+                streams[0].wait_stream(torch.cuda.current_stream())
+                res = s.step()
+            torch.cuda.current_stream().wait_stream(streams[0])
+            want.append([t.clone() for t in res[:3]] + s.state())
+            s.restore(keep)
+        torch.cuda.synchronize()
+        for graph, st in zip(graphs, streams):         # at the same time
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for s, o, w in zip(servers, outs, want):
+            for got, ref in zip(list(o[:3]) + s.state(), w):
+                assert torch.equal(got.view(torch.uint8) if got.is_floating_point() else got,
+                                   ref.view(torch.uint8) if ref.is_floating_point() else ref)
+    from dkernel_b200 import _lib
+    assert _lib.wait_status() == 0
+
+
+CHILD = r"""
+import hashlib, json, sys
+sys.path[:0] = [%(root)r, %(root)r + "/tests"]
+import torch
+import test_paged_gpu as t
+from dkernel_b200 import _lib
+from paged_cases import local_stride, paged_inputs, random_pattern
+out = {}
+def run(name, x, pat, bs, single=False):
+    o, l = t.call(t.module(bs, pat, seq_dim=x["seq_dim"], impl="sm100"), x, single=single, return_lse=True)
+    h = hashlib.md5(torch.nan_to_num(o.float()).cpu().numpy().tobytes())
+    h.update(torch.nan_to_num(l, neginf=-1e30).cpu().numpy().tobytes())
+    out[name] = h.hexdigest()
+bf16, f16 = torch.bfloat16, torch.float16
+ctx, new = [0, 63, 500, 333, 900], [64, 3, 40, 0, 61]
+run("trees", paged_inputs(1, 8, 2, 128, ctx, new, 16, bf16), local_stride(2, 16, 3, 4), 64)
+run("e4m3", paged_inputs(2, 8, 2, 128, ctx, new, 32, bf16, fp8=True), local_stride(2, 16, 3, 4), 64)
+run("rows", paged_inputs(3, 6, 2, 64, ctx, new, 8, f16), random_pattern(6, 16, 0.3, 2), 64)
+run("small", paged_inputs(4, 4, 4, 96, ctx, new, 16, f16), random_pattern(4, 64, 0.3, 2), 16)
+run("chains", paged_inputs(5, 20, 1, 64, [0, 70, 300], [300, 129, 7], 64, bf16, tree=False), local_stride(1, 16, 3, 4), 64)
+run("tokens", paged_inputs(6, 8, 2, 128, [0, 64, 1000], [1, 1, 1], 16, bf16, fp8=True, tree=False), local_stride(2, 16, 3, 4), 64, True)
+x = paged_inputs(7, 4, 2, 64, [200, 130], [20, 30], 16, bf16)
+x["table"][0, 3] = -1; x["table"][1, 5] = 10 ** 6
+run("missing", x, local_stride(2, 8, 2, 2), 64)
+torch.cuda.synchronize()
+print(json.dumps(dict(status=_lib.wait_status(), lib=_lib.LIB_PATH, out=out)))
+"""
+
+
+def test_checking_build_runs_clean():
+    """The same calls through the release and the bounds-checking library: no check fires, the outputs are the same bits."""
+    import json
+    import os
+    import subprocess
+    import sys
+    from dkernel_b200 import _build
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    got = []
+    for lib in (_build.LIB, _build.LIB_DEBUG):
+        assert os.path.exists(lib)
+        r = subprocess.run([sys.executable, "-c", CHILD % dict(root=root)], capture_output=True, text=True, timeout=300,
+                           env={**os.environ, "BSA_B200_LIB": lib})
+        assert r.returncode == 0, r.stdout + r.stderr
+        got.append(json.loads(r.stdout.strip().splitlines()[-1]))
+    assert got[0]["status"] == got[1]["status"] == 0
+    assert got[0]["lib"] != got[1]["lib"] and got[0]["out"] == got[1]["out"]

@@ -1183,19 +1183,23 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint8_t* src = raw + rs * Geo::kRawTile;
         uint8_t* dst = tile + s * kTile;
         // 16 values a lane and turn, the two warps in turns.  A lane keeps its place in the row, and its rows are 8 apart, so
-        // that its addresses are a base and constants; upper sub-tiles store their odd half first: no bank twice
+        // that its addresses are a base and constants.  At D = 128 eight lanes take half of a row and the other half of its
+        // neighbour: no bank twice, neither in the loads (rows of 128 bytes) nor in the stores (16-byte pieces 0, 2, 4, 6,
+        // exclusive-or the row)
         constexpr int kPieces = D / 16, kRows = 32 / kPieces;          // 4 or 8 rows a turn
-        const int row = (warp - kWConv) * kRows + lane / kPieces, pc = lane % kPieces, odd = pc >> 2, c0 = (pc & 3) * 2;
-        const uint8_t* from = src + ((warp - kWConv) * 32 + lane) * 16;
-        uint8_t* base = dst + odd * 8192 + row * 128;
-        const int a0 = ((c0 + odd) ^ (row & 7)) * 16, a1 = ((c0 + 1 - odd) ^ (row & 7)) * 16;
+        const int set = lane >> 3, low = (lane >> 2) & 1;
+        const int row = (warp - kWConv) * kRows + (D == 64 ? lane >> 2 : (set & 2) + ((set ^ low) & 1));
+        const int pc = D == 64 ? lane & 3 : low * 4 + (lane & 3), c0 = (pc & 3) * 2;
+        const uint8_t* from = src + row * D + pc * 16;
+        uint8_t* base = dst + (pc >> 2) * 8192 + row * 128;
+        const int a0 = (c0 ^ (row & 7)) * 16, a1 = ((c0 + 1) ^ (row & 7)) * 16;
         // Turns go four at a time, their loads before any store: the compiler cannot tell the tiles apart and would wait
         // for each turn's load (1000 cycles a tile of 64 x 128)
 #pragma unroll
         for (int q0 = 0; q0 < 32 / kRows; q0 += 4) {
           uint4 v[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const uint4*>(from + (q0 + q) * 1024);
+          for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const uint4*>(from + (q0 + q) * 2 * kRows * D);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const uint32_t in[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
@@ -1205,9 +1209,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               out[2 * i] = e4m3x2_to_f16((uint16_t)in[i]);
               out[2 * i + 1] = e4m3x2_to_f16((uint16_t)(in[i] >> 16));
             }
-            const uint4 lo = make_uint4(out[0], out[1], out[2], out[3]), hi = make_uint4(out[4], out[5], out[6], out[7]);
-            *reinterpret_cast<uint4*>(base + (q0 + q) * 2 * kRows * 128 + a0) = odd ? hi : lo;
-            *reinterpret_cast<uint4*>(base + (q0 + q) * 2 * kRows * 128 + a1) = odd ? lo : hi;
+            *reinterpret_cast<uint4*>(base + (q0 + q) * 2 * kRows * 128 + a0) = make_uint4(out[0], out[1], out[2], out[3]);
+            *reinterpret_cast<uint4*>(base + (q0 + q) * 2 * kRows * 128 + a1) = make_uint4(out[4], out[5], out[6], out[7]);
           }
         }
         fence_proxy_async();

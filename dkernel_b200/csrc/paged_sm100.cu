@@ -681,11 +681,12 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            tc_mma_ts(tO, tS + sb * 64 + kk * 8, vd + (uint64_t)((kk * 2048) >> 4), idesc_pv, kk ? 1u : acc0);
+            tc_mma_ts(tO, tS + sb * 64 + (split ? (kk >> 1) * 32 + (kk & 1) * 8 : kk * 8), vd + (uint64_t)((kk * 2048) >> 4),
+                      idesc_pv, kk ? 1u : acc0);
           if (split) {
 #pragma unroll
-            for (int kk = 4; kk < 8; ++kk)    // the low terms of P
-              tc_mma_ts(tO, tS + sb * 64 + kk * 8, vd + (uint64_t)(((kk & 3) * 2048) >> 4), idesc_pv, 1u);
+            for (int kk = 0; kk < 4; ++kk)    // the low terms of P, 16 columns behind the high ones of the same 32 keys
+              tc_mma_ts(tO, tS + sb * 64 + (kk >> 1) * 32 + 16 + (kk & 1) * 8, vd + (uint64_t)((kk * 2048) >> 4), idesc_pv, 1u);
           }
           tc_commit(&tl->pv_done[sb]);
           tc_commit(&tl->v_free[s]);
@@ -800,29 +801,33 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       auto softmax_tile = [&](auto cw, uint64_t M, uint32_t tSb) -> bool {
         constexpr int CW = decltype(cw)::value;
         static_assert(CW == 64 || CW == 16, "whole tiles or quarters");
-        constexpr int kHalf = CW == 64 ? 32 : CW;           // keys between two stores
+        // 32 logits at a time, read once for the maximum and once more for the weights: half the code of all 64 at once
+        // (instruction fetch is a fifth of this kernel's stalls) and half the registers
+        constexpr int BL = CW == 64 ? 32 : 16;
         const int c0 = CW == 64 ? 0 : rep * CW;
-        uint32_t sv[CW];
-        if constexpr (CW == 64) {
-          tmem_ld32(tSb, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
-          tmem_ld32(tSb + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
-        } else {
-          tmem_ld16(tSb + c0, sv);
-        }
-        tmem_ld_wait();
         const uint64_t mc = CW == 64 ? M : (M >> c0) & low_bits(CW);
-        const bool att = mc != 0ull;
-        if (__any_sync(0xffffffffu, mc != low_bits(CW))) {
-          const uint32_t lo = (uint32_t)mc, hi = (uint32_t)(mc >> 32);
+        const bool att = mc != 0ull, masked = __any_sync(0xffffffffu, mc != low_bits(CW));
+        uint32_t sv[BL];
+        auto logits = [&](int h) {
+          if constexpr (CW == 64) tmem_ld32(tSb + h * 32, sv);
+          else tmem_ld16(tSb + c0, sv);
+          tmem_ld_wait();
+          if (masked) {
+            const uint32_t m32 = (uint32_t)(mc >> (h * 32));
 #pragma unroll
-          for (int c = 0; c < CW; ++c)
-            if (!(((c < 32 ? lo : hi) >> (c & 31)) & 1u)) sv[c] = 0xff800000u;
-        }
+            for (int c = 0; c < BL; ++c)
+              if (!((m32 >> c) & 1u)) sv[c] = 0xff800000u;
+          }
+        };
         float mt[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int h = 0; h < CW / BL; ++h) {
+          logits(h);
 #pragma unroll
-        for (int c = 0; c < CW; c += 8)
+          for (int c = 0; c < BL; c += 8)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mt[i] = pmax3(mt[i], __uint_as_float(sv[c + 2 * i]), __uint_as_float(sv[c + 2 * i + 1]));
+            for (int i = 0; i < 4; ++i) mt[i] = pmax3(mt[i], __uint_as_float(sv[c + 2 * i]), __uint_as_float(sv[c + 2 * i + 1]));
+        }
         const float mx = fmaxf(pmax3(mt[0], mt[1], mt[2]), mt[3]) * scale2;
         float alpha = 1.f;
         bool need = false;
@@ -841,30 +846,32 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const float neg_m = kShift - m_used;
         const uint64_t scale_2 = f32x2(scale2, scale2), neg_m2 = f32x2(neg_m, neg_m);
         uint64_t sum2[2] = {0ull, 0ull};
-#pragma unroll
-        for (int h = 0; h < CW / kHalf; ++h) {
-          uint32_t pk[kHalf / 2], pq[kHalf / 2];
+#pragma unroll 1
+        for (int h = 0; h < CW / BL; ++h) {
+          if (CW == 64) logits(h);            // a quarter's are still there
+          uint32_t pk[BL / 2], pq[BL / 2];
           if (live) {
 #pragma unroll
-            for (int c = 0; c < kHalf / 2; ++c) {
+            for (int c = 0; c < BL / 2; ++c) {
               float x0, x1;
-              f32x2_split(fma_f32x2(f32x2(sv[h * 32 + 2 * c], sv[h * 32 + 2 * c + 1]), scale_2, neg_m2), x0, x1);
+              f32x2_split(fma_f32x2(f32x2(sv[2 * c], sv[2 * c + 1]), scale_2, neg_m2), x0, x1);
               const float p0 = pex2(x0), p1 = pex2(x1);
               sum2[c & 1] = add_f32x2(sum2[c & 1], f32x2(p0, p1));
               psplit<BE>(p0, p1, pk[c], pq[c]);
             }
           } else {
 #pragma unroll
-            for (int c = 0; c < kHalf / 2; ++c) pk[c] = pq[c] = 0u;
+            for (int c = 0; c < BL / 2; ++c) pk[c] = pq[c] = 0u;
           }
           if constexpr (CW == 64) {
-            tmem_st16(tSb + h * 16, pk);
-            tmem_st16(tSb + 32 + h * 16, pq);
+            // both terms over the logits that they come from, so that the other half is still there
+            tmem_st16(tSb + h * 32, pk);
+            tmem_st16(tSb + h * 32 + 16, pq);
           } else {
             // this repetition's keys, and no weight on the others'
-            uint32_t z[kHalf / 2];
+            uint32_t z[BL / 2];
 #pragma unroll
-            for (int c = 0; c < kHalf / 2; ++c) {
+            for (int c = 0; c < BL / 2; ++c) {
               z[c] = 0u;
               if (lane >= 16) pk[c] = pq[c];
             }

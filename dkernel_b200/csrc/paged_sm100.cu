@@ -1386,11 +1386,14 @@ int launch_paged(const bsa_paged_params* p, const PagedShape& shape, cudaStream_
   if (rc) return rc;
   constexpr int eb = KV8 ? 1 : 2;
   const uint32_t box_d = KV8 ? D : 64;
+  // no more than a head's row at once: what lies behind it is another head's, for another CTA and time (with 256 bytes for
+  // rows of 128, an e4m3 cache's DRAM reads doubled)
+  const int promotion = p->d * eb >= 256 ? 256 : p->d * eb >= 128 ? 128 : 64;
   rc = make_tmap_4d(&tmK, p->k_cache, eb, p->d, p->page_size, p->hkv, p->num_pages, p->kc_ss * eb, p->kc_sh * eb, p->kc_sp * eb,
-                    box_d, sh.box, !KV8, BF16);
+                    box_d, sh.box, !KV8, BF16, promotion);
   if (rc) return rc;
   rc = make_tmap_4d(&tmV, p->v_cache, eb, p->d, p->page_size, p->hkv, p->num_pages, p->vc_ss * eb, p->vc_sh * eb, p->vc_sp * eb,
-                    box_d, sh.box, !KV8, BF16);
+                    box_d, sh.box, !KV8, BF16, promotion);
   if (rc) return rc;
   int dev = 0, sms = 0;
   BSA_CHECK_CUDA(cudaGetDevice(&dev));

@@ -27,7 +27,7 @@ struct Tmap4 {
 int make_tmap_4d(Tmap4* out, const void* base, int elem_bytes, uint64_t d, uint64_t seq,
                  uint64_t heads, uint64_t batch, int64_t seq_stride_b, int64_t head_stride_b,
                  int64_t batch_stride_b, uint32_t box_d, uint32_t box_seq, bool swizzle128,
-                 bool is_bf16);
+                 bool is_bf16, int l2_promotion = 256);   // bytes that L2 fetches at a time: 256, 128 or 64
 
 // 3-D tiled map of a packed (tokens, heads, d) tensor of a 16-bit type, 128-byte swizzled boxes of
 // box_tokens x box_heads x 64; strides in bytes, token_stride >= head_stride.

@@ -82,7 +82,7 @@ bool tma_compatible(const void* base, int elem_bytes, int64_t ss, int64_t sh, in
 int make_tmap_4d(Tmap4* out, const void* base, int elem_bytes, uint64_t d, uint64_t seq,
                  uint64_t heads, uint64_t batch, int64_t seq_stride_b, int64_t head_stride_b,
                  int64_t batch_stride_b, uint32_t box_d, uint32_t box_seq, bool swizzle128,
-                 bool is_bf16) {
+                 bool is_bf16, int l2_promotion) {
   auto enc = get_encode();
   if (!enc) {
     set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
@@ -129,7 +129,10 @@ int make_tmap_4d(Tmap4* out, const void* base, int elem_bytes, uint64_t d, uint6
   CUresult r = enc(&out->map, dt, 4, const_cast<void*>(base), gdim, gstr, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE,
                    swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   l2_promotion >= 256   ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                   : l2_promotion >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                         : CU_TENSOR_MAP_L2_PROMOTION_L2_64B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with CUresult %d (dims %llu,%llu,%llu,%llu strides "
               "%llu,%llu,%llu box %u,%u,%u,%u)",

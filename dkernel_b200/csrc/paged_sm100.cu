@@ -16,6 +16,15 @@
 // A K/V tile is 64 tokens = 1, 2 or 4 pattern blocks, wherever their pages are: one TMA box per page piece.
 // Warps (192 threads, 256 with an e4m3 cache): 0-3 softmax and epilogue, 4 planner and TMA producer, 5 MMA issuer,
 // 6 and 7 e4m3 -> f16.  TMEM: S 2x64 | O 128 columns.
+//
+// Measured (bf16, 32 / 8 heads of 128, blocks of 64, band of 16 + one column in 8; one call after another, which brings the
+// card to its power limit and 1.6 GHz): 64 single tokens over 1024..8192 tokens 91 us (4.3 TB/s of attended bytes, 84 us before
+// the limit is reached), 64 trees of 15..29 drafts 126 us, 48 trees of 30..60 on an e4m3 cache 203 us, one token over 4000
+// 22 us.  A launch's first 9 us go by until its first tile is there: tables and lists, each instruction met for the first
+// time; then single tokens run at what HBM gives, wide trees at the pace of the softmax warps (two per scheduler: 1850
+// cycles a tile against 1024 of exponentials), with shared memory three quarters busy (Q, K and twice V as operands).
+// The cost of a join: 2 to 8 us.  K/V tiles pass through L2 evict-first: without that this code and the tables are fetched
+// from DRAM again, launch after launch, and trees take 10 % more.
 #include <type_traits>
 
 #include "ptx.cuh"
@@ -30,7 +39,7 @@ constexpr int kSegPages = 128;        // and pages of theirs
 constexpr int kWindow = 128;          // columns whose union is formed at a time
 constexpr uint32_t kTailFlag = 1u << 31;
 constexpr uint32_t kColMask = (1u << 23) - 1u;   // bits 23..30: pages that exist
-constexpr int kOverhead = 3;          // an item's fixed cost in K/V tiles
+constexpr int kOverhead = 3;          // an item's fixed cost in K/V tiles (2: trees 1 % slower; 4, 6: single tokens 1, 2 %)
 constexpr float kRescale = 8.0f;
 constexpr int kWPlan = 4, kWIssue = 5, kWConv = 6;
 
@@ -186,8 +195,9 @@ __device__ __forceinline__ Entry entry_of(const PagedShape& sh, int e, int nE, i
 }
 
 // ------------------------------------------------------------------ the kernel
-// P is kept as the sum of two 16-bit terms side by side in S's columns, as in the decode and the long packed kernels:
-// no precision hangs on which weights a 16-bit type holds exactly.
+// P is kept as the sum of two 16-bit terms in S's columns, as in the decode and the long packed kernels: no precision
+// hangs on which weights a 16-bit type holds exactly (the output is as far from 64 bits as its own rounding makes it; one
+// term would add as much again, for a few percent of time: with half of the products left out, trees take 119 us, not 126).
 template <bool BF16, int D, int BS, bool KV8>
 __global__ void __launch_bounds__(PGeo<D, KV8>::kThreads, 2)
 paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ Tmap4 tmK, const __grid_constant__ Tmap4 tmV,
@@ -609,7 +619,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               pl->page[at * per_entry + z] = pg;
               have |= (pg >= 0 ? 1u : 0u) << z;
             }
-            pl->col[at] = (uint32_t)col | have << 23 | tail;
+            pl->col[at] = ((uint32_t)col & kColMask) | have << 23 | tail;
             pl->fl[at] = fl;
             if (tail || have != all_pages || fl != all_rows) atomicOr(&pl->special[at >> 5], 1u << (at & 31));
           }

@@ -55,7 +55,8 @@ def plan_paged_step(block_tables: Tensor, page_counts: Tensor, free_pages: Tenso
     stack ``free_pages[:num_free]`` in the order of request and page, missing ones popped from its top in that order.
     Updated in place, all int32: ``block_tables`` (batch, pages per request), ``page_counts`` (batch,),
     ``free_pages`` (any size that holds all pages), ``num_free`` (1,).  Where the stack runs empty the table gets -1,
-    the tokens have slot -1 and ``short`` counts the missing pages; a later step gets them once pages are free.
+    the tokens have slot -1 (their keys and values are stored nowhere) and ``short`` counts the missing pages; a later step
+    with the same lengths gets them once pages are free.
     ``max_new_tokens`` is the size of the packed batch: outputs behind the last request are slot -1, position 0, and
     new tokens past it are dropped.  With ``tree_mask`` (max_new_tokens,) int64, see ``SparseAttention.forward``, a
     position is the context's length plus the number of other drafts attended, else they count up."""

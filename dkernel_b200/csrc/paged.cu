@@ -229,7 +229,8 @@ template <typename T> __device__ __forceinline__ uint16_t to_e4m3x2(T x, T y, fl
 // Both caches in one grid: blockIdx.y = 0 for K, 1 for V.  Bound by HBM: each element is read and written once.  A
 // thread moves VEC elements (16 bytes of the cache, or of the input where that is wider, if everything is aligned; else
 // one), 64 bytes at a time so that enough loads are in flight; consecutive threads are consecutive in (token, head, dim).
-// 65000 tokens x 8 heads x 128 from bf16 into e4m3: 85 us, 4.7 TB/s (with 124 registers, two CTAs per SM, 119).
+// 65000 tokens x 8 heads x 128 from bf16 into e4m3: 80 us, 5.0 TB/s (119 with 124 registers, two CTAs per SM; 84 to 100
+// with more CTAs than are resident).
 template <typename T, typename C, int VEC>
 __global__ void __launch_bounds__(256, 4) paged_write_kernel(const __grid_constant__ bsa_paged_write_params p, const FastDiv per_token,
                                                           const FastDiv pieces, const FastDiv page, uint32_t total) {
@@ -419,7 +420,7 @@ int launch_write_vec(const bsa_paged_write_params* p, cudaStream_t s) {
     return BSA_E_TOOBIG;
   }
   const int64_t per_cta = 256 * (VEC * sizeof(T) > 16 ? 2 : 4);
-  const unsigned grid = (unsigned)std::min<int64_t>((total + per_cta - 1) / per_cta, 148 * 16);
+  const unsigned grid = (unsigned)std::min<int64_t>((total + per_cta - 1) / per_cta, 148 * 2);   // all resident
   paged_write_kernel<T, C, VEC><<<dim3(grid, 2), 256, 0, s>>>(*p, FastDiv((uint32_t)per_token), FastDiv(p->d / VEC),
                                                                FastDiv(p->page_size), (uint32_t)total);
   return check_launch("paged_write_kernel");

@@ -108,6 +108,12 @@ template <int NK, int NV, int NR> struct PTail {
   alignas(16) float stage[2048];             // parts of some columns; without repetitions: 32 rows x 64 bytes per warp
 };
 
+// Bounded like every wait, but by 10 s: a warp that recomputes the rows that a NaN got into (32 of them, 6 ms each over
+// 64 thousand attended keys) keeps the others waiting that long.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return mbar_wait(bar, parity, status, code, 10000000000ull);
+}
+
 __device__ __forceinline__ float pex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -464,7 +470,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         bool first = true, begins = true;
         auto open = [&]() {
           const int pb = k & 1;
-          if (!mbar_wait(&tl->plan_free[pb], ((k >> 1) & 1) ^ 1, wait_status, 1001)) { ok = false; return; }
+          if (!wait_for(&tl->plan_free[pb], ((k >> 1) & 1) ^ 1, wait_status, 1001)) { ok = false; return; }
           pl = &tl->plan[pb];
           pl->tb[lane] = my_tb;
           if (lane < 8) pl->dm[lane] = my_dm;
@@ -494,7 +500,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const uint32_t x = rg + (uint32_t)j;
             const int s = is_v ? x % NLV : x % NLK;
             uint64_t* full = (is_v ? vf : kf) + s;
-            if (!mbar_wait((is_v ? ve : ke) + s, ((is_v ? x / NLV : x / NLK) & 1) ^ 1, wait_status, is_v ? 1014 : 1013)) { ok = false; break; }
+            if (!wait_for((is_v ? ve : ke) + s, ((is_v ? x / NLV : x / NLK) & 1) ^ 1, wait_status, is_v ? 1014 : 1013)) { ok = false; break; }
             if (lane == 0) mbar_expect_tx(full, kLoadBytes);
             __syncwarp();
             if (lane < per * subs) {
@@ -512,7 +518,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             __syncwarp();
             if (t == 0 && begins) {
               // Q behind the first K
-              if (items > 0 && !mbar_wait(&tl->q_free, (items - 1) & 1, wait_status, 1012)) { ok = false; break; }
+              if (items > 0 && !wait_for(&tl->q_free, (items - 1) & 1, wait_status, 1012)) { ok = false; break; }
               ++items;
               const int pos = 128 / sh.cr, boxes = kSub * pos;
               if (lane == 0) mbar_expect_tx(&tl->q_full, (uint32_t)(boxes * sh.ct * sh.gt * 128));
@@ -629,7 +635,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     if (ok) {
       const int pb = k & 1;
-      if (mbar_wait(&tl->plan_free[pb], ((k >> 1) & 1) ^ 1, wait_status, 1002)) {
+      if (wait_for(&tl->plan_free[pb], ((k >> 1) & 1) ^ 1, wait_status, 1002)) {
         if (lane == 0) {
           tl->plan[pb].valid = -1;
           mbar_arrive(&tl->plan_full[pb]);
@@ -649,20 +655,20 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     bool ok = true, started = false;
     for (int k = 0; ok; ++k) {
       const int pb = k & 1;
-      if (!mbar_wait(&tl->plan_full[pb], (k >> 1) & 1, wait_status, 1021)) break;
+      if (!wait_for(&tl->plan_full[pb], (k >> 1) & 1, wait_status, 1021)) break;
       const PPlan* pl = &tl->plan[pb];
       if (pl->valid < 0) break;
       const int nt = pl->nt, last = pl->last;
       const bool split = pl->rr == 128;       // both terms of P in a row; else they have rows of their own
       if (pl->first) {
-        if (!mbar_wait(QCONV ? &tl->q_ready : &tl->q_full, items & 1, wait_status, 1022)) break;
+        if (!wait_for(QCONV ? &tl->q_ready : &tl->q_full, items & 1, wait_status, 1022)) break;
         ++items;
         started = false;
       }
       auto qk = [&](int j) -> bool {
         const uint32_t x = g + (uint32_t)j;
         const int s = x % NK, sb = x & 1;
-        if (!mbar_wait(&tl->k_full[s], (x / NK) & 1, wait_status, 1023)) return false;
+        if (!wait_for(&tl->k_full[s], (x / NK) & 1, wait_status, 1023)) return false;
         tc_fence_after();
         const uint64_t kd = kdesc + (uint64_t)((s * kTile) >> 4);
         if (elect_one()) {
@@ -681,10 +687,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int j = 0; ok && j < nt; ++j) {
         const uint32_t x = g + (uint32_t)j;
         const int s = x % NV, sb = x & 1;
-        if (!mbar_wait(&tl->v_full[s], (x / NV) & 1, wait_status, 1024)) { ok = false; break; }
-        if (!mbar_wait(&tl->p_full[sb], (x >> 1) & 1, wait_status, 1025)) { ok = false; break; }
+        if (!wait_for(&tl->v_full[s], (x / NV) & 1, wait_status, 1024)) { ok = false; break; }
+        if (!wait_for(&tl->p_full[sb], (x >> 1) & 1, wait_status, 1025)) { ok = false; break; }
         // the item before has read O
-        if (!started && items > 1 && !mbar_wait(&tl->o_free, (items - 2) & 1, wait_status, 1026)) { ok = false; break; }
+        if (!started && items > 1 && !wait_for(&tl->o_free, (items - 2) & 1, wait_status, 1026)) { ok = false; break; }
         tc_fence_after();
         const uint64_t vd = vdesc + (uint64_t)((s * kTile) >> 4);
         const uint32_t acc0 = started ? 1u : 0u;
@@ -726,7 +732,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     auto meet = [&]() -> bool {
       __syncwarp();
       if (lane == 0) mbar_arrive(&tl->met);
-      return mbar_wait(&tl->met, meets++ & 1, wait_status, 1036);
+      return wait_for(&tl->met, meets++ & 1, wait_status, 1036);
     };
     // the row's own state over an item
     float m_used = -INFINITY, l = 0.f;
@@ -740,7 +746,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int k = -1; alive; ++k) {
       const bool dry = k < 0;
       const int pb = k & 1;
-      if (!dry && !mbar_wait(&tl->plan_full[pb], (k >> 1) & 1, wait_status, 1031)) break;
+      if (!dry && !wait_for(&tl->plan_full[pb], (k >> 1) & 1, wait_status, 1031)) break;
       const PPlan* pl = dry ? static_cast<const PPlan*>(&tl->warm) : &tl->plan[pb];   // nothing behind the head is read then
       if (pl->valid < 0) break;
       const int nt = pl->nt, n = pl->n, rr = pl->rr;
@@ -778,7 +784,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         if (QCONV && !dry) {
           // this thread's row of Q from bf16 to f16, where it lies
-          if (!mbar_wait(&tl->q_full, q_items & 1, wait_status, 1038)) break;
+          if (!wait_for(&tl->q_full, q_items & 1, wait_status, 1038)) break;
           ++q_items;
           uint32_t big = 0;
 #pragma unroll 1
@@ -899,7 +905,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
         if (any && mine > 0) {
           // rows whose maximum moved: rescale their O once the product before has landed
-          if (!mbar_wait(&tl->pv_done[(gs - 1) & 1], ((gs - 1) >> 1) & 1, wait_status, 1034)) return false;
+          if (!wait_for(&tl->pv_done[(gs - 1) & 1], ((gs - 1) >> 1) & 1, wait_status, 1034)) return false;
           tc_fence_after();
 #pragma unroll 1
           for (int ch = 0; ch < D / 16; ++ch) {
@@ -953,13 +959,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           any_att = __any_sync(0xffffffffu, row_ok && M != 0ull);
           if (!row_ok) M = ~0ull;             // nobody reads these rows: nothing to mask
         }
-        if (!dry && !mbar_wait(&tl->qk_done[sb], (gs >> 1) & 1, wait_status, 1032)) { alive = false; break; }
+        if (!dry && !wait_for(&tl->qk_done[sb], (gs >> 1) & 1, wait_status, 1032)) { alive = false; break; }
         tc_fence_after();
         if (clear) {
           // keys behind the item's end: P is 0 there, and 0 times whatever the page holds has to be 0, too
           // (two V slots at least: this tile's barrier cannot still be in the phase of the tile before in its slot, whose
           // product was over before this tile's logits were there)
-          if (!mbar_wait(&tl->v_full[s], (gs / NV) & 1, wait_status, 1033)) { alive = false; break; }
+          if (!wait_for(&tl->v_full[s], (gs / NV) & 1, wait_status, 1033)) { alive = false; break; }
           uint8_t* vt = sV + s * kTile;
           const int cend = (clear0 / BS + 1) * BS;
           for (int q = r; q < (cend - clear0) * kSub * 8; q += 128) {
@@ -991,7 +997,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (!alive) break;
       if (pl->last) {
         // ---- the item's result
-        if (!dry && !mbar_wait(&tl->pv_done[(gs - 1) & 1], ((gs - 1) >> 1) & 1, wait_status, 1035)) break;
+        if (!dry && !wait_for(&tl->pv_done[(gs - 1) & 1], ((gs - 1) >> 1) & 1, wait_status, 1035)) break;
         tc_fence_after();
         const int part = pl->part;
         const int item_row = (i_tok - pl->tok0) * sh.gt + head - pl->head0;
@@ -1178,7 +1184,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     uint32_t rg = 0;
     for (int k = 0;; ++k) {
       const int pb = k & 1;
-      if (!mbar_wait(&tl->plan_full[pb], (k >> 1) & 1, wait_status, 1041)) break;
+      if (!wait_for(&tl->plan_full[pb], (k >> 1) & 1, wait_status, 1041)) break;
       const PPlan* pl = &tl->plan[pb];
       if (pl->valid < 0) break;
       const int nt = pl->nt;
@@ -1195,8 +1201,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         uint64_t* empty = is_v ? tl->v_free : tl->k_free;
         uint64_t* rf = is_v ? tl->raw_v_full : tl->raw_k_full;
         uint64_t* re = is_v ? tl->raw_v_free : tl->raw_k_free;
-        if (!mbar_wait(&rf[rs], (x / NR) & 1, wait_status, is_v ? 1044 : 1042)) { ok = false; break; }
-        if (!mbar_wait(&empty[s], ((is_v ? x / NV : x / NK) & 1) ^ 1, wait_status, is_v ? 1045 : 1043)) { ok = false; break; }
+        if (!wait_for(&rf[rs], (x / NR) & 1, wait_status, is_v ? 1044 : 1042)) { ok = false; break; }
+        if (!wait_for(&empty[s], ((is_v ? x / NV : x / NK) & 1) ^ 1, wait_status, is_v ? 1045 : 1043)) { ok = false; break; }
         const uint8_t* src = raw + rs * Geo::kRawTile;
         uint8_t* dst = tile + s * kTile;
         // 16 values a lane and turn, the two warps in turns.  A lane keeps its place in the row, and its rows are 8 apart, so

@@ -812,3 +812,16 @@ def test_checking_build_runs_clean():
         got.append(json.loads(r.stdout.strip().splitlines()[-1]))
     assert got[0]["status"] == got[1]["status"] == 0
     assert got[0]["lib"] != got[1]["lib"] and got[0]["out"] == got[1]["out"]
+
+
+def test_many_rows_that_a_nan_reaches():
+    """Every row of a long context attends a NaN: all are recomputed, none of the kernel's waits gives up meanwhile."""
+    from dkernel_b200 import _lib
+    hq, hkv, d, page, n, L = 4, 1, 64, 64, 64, 16000
+    mod = module(64, np.tril(np.ones((1, 256, 256))), seq_dim=1, impl="sm100")
+    x = paged_inputs(2, hq, hkv, d, [L], [n], page, bf16)
+    x["v"][x["table"][0, 100], 5] = float("nan")
+    out, lse = call(mod, x, return_lse=True)
+    torch.cuda.synchronize()
+    assert _lib.wait_status() == 0
+    assert torch.isnan(out).all() and torch.isfinite(lse).all()

@@ -119,9 +119,10 @@ __device__ __forceinline__ float pex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// NaN if one of them is: a tile whose attended logits are all NaN must not look like one without attended keys
 __device__ __forceinline__ float pmax3(float a, float b, float c) {
   float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 template <bool BF16> __device__ __forceinline__ uint32_t ppack2(float lo, float hi) {
@@ -844,7 +845,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int i = 0; i < 4; ++i) mt[i] = pmax3(mt[i], __uint_as_float(sv[c + 2 * i]), __uint_as_float(sv[c + 2 * i + 1]));
         }
-        const float mx = fmaxf(pmax3(mt[0], mt[1], mt[2]), mt[3]) * scale2;
+        const float mx = pmax3(pmax3(mt[0], mt[1], mt[2]), mt[3], mt[3]) * scale2;     // NaN stays in m_used and in l
         float alpha = 1.f;
         bool need = false;
         if (mx != -INFINITY) {

@@ -75,9 +75,10 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// NaN if one of them is: a block whose attended logits are all NaN must not look like one without attended keys
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 template <bool BF16>
@@ -622,7 +623,7 @@ fwd_persist_kernel(const __grid_constant__ Tmap4 tmQ, const __grid_constant__ Tm
               for (int i = 0; i < 4; ++i)
                 m4[i] = max3(m4[i], __uint_as_float(sv[c + 2 * i]), __uint_as_float(sv[c + 2 * i + 1]));
             mx = max3(max3(m4[0], m4[1], m4[2]), max3(m4[3], __uint_as_float(sv[60]), __uint_as_float(sv[61])),
-                      fmaxf(__uint_as_float(sv[62]), __uint_as_float(sv[63]))) * scale2;
+                      max3(__uint_as_float(sv[62]), __uint_as_float(sv[63]), __uint_as_float(sv[63]))) * scale2;
           }
         }
         float alpha = 1.f;
@@ -754,7 +755,7 @@ fwd_persist_kernel(const __grid_constant__ Tmap4 tmQ, const __grid_constant__ Tm
               *reinterpret_cast<uint2*>(orow + ch * 64 + i * 8) = make_uint2(w[2 * i], w[2 * i + 1]);
         }
       }
-      if (row_ok && lse_ptr) *lse_ptr = l > 0.f ? (m_used - kShift + log2f(l)) * kLn2 : -INFINITY;
+      if (row_ok && lse_ptr) *lse_ptr = l == 0.f ? -INFINITY : (m_used - kShift + log2f(l)) * kLn2;   // NaN stays
       __syncwarp();
       if (lane == 0) mbar_arrive(&tl->plan_free[pb]);
       ++k;

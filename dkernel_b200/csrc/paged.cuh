@@ -7,10 +7,12 @@
 
 namespace bsa {
 
-struct PagedRequest { int t0, n, L; };   // first query row, drafted tokens, context tokens
+// first query row, drafted tokens, context tokens; false: nothing is stored, whatever pages the block table names
+struct PagedRequest { int t0, n, L; bool stored = true; };
 
-// Query rows stay inside [0, total_q) whatever cu_q holds; a request that stores fewer tokens than it
-// queries counts as one without context.
+// Query rows stay inside [0, total_q) whatever cu_q holds.  A request that stores nothing has rows that attend nothing
+// (batches are padded with such requests); one that stores some tokens, but fewer than it queries, counts as one without
+// context.
 __device__ __forceinline__ PagedRequest paged_request(const bsa_paged_params& p, int b) {
   PagedRequest r;
   if (p.cu_q) {
@@ -20,7 +22,9 @@ __device__ __forceinline__ PagedRequest paged_request(const bsa_paged_params& p,
     r.t0 = b;
     r.n = 1;
   }
-  r.L = max(__ldg(p.seqlens + b) - r.n, 0);
+  const int stored = __ldg(p.seqlens + b);
+  r.stored = stored > 0;
+  r.L = max(stored - r.n, 0);
   return r;
 }
 
@@ -77,7 +81,7 @@ __device__ __noinline__ void paged_row(const bsa_paged_params& p, int b, PagedRe
     int64_t vrow = 0;
     float x = -INFINITY;
     if (on) {
-      const int pg = page_of(table, s / p.page_size, p.max_pages, p.num_pages);
+      const int pg = page_of(table, s / p.page_size, r.stored ? p.max_pages : 0, p.num_pages);
       on = pg >= 0;
       if (on) {
         const int slot = (int)(s % p.page_size);

@@ -622,7 +622,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             uint32_t have = 0;
 #pragma unroll 1
             for (int z = 0; z < per_entry; ++z) {
-              const int pg = page_of(table, s0 + z, p.max_pages, p.num_pages);
+              const int pg = page_of(table, s0 + z, r.stored ? p.max_pages : 0, p.num_pages);
               pl->page[at * per_entry + z] = pg;
               have |= (pg >= 0 ? 1u : 0u) << z;
             }

@@ -161,7 +161,8 @@ class SparseAttention(torch.nn.Module):
         Another: with ``block_tables`` (batch, pages per request) int32, ``k`` and ``v`` are paged caches,
         (pages, page size, kv heads, dim), or (pages, kv heads, page size, dim) for ``seq_dim=2``, in q's
         type or e4m3, and q is packed (tokens, heads, dim).  ``seqlens`` (batch,) counts the stored tokens
-        of each request, its query tokens' own included (see :func:`dkernel_b200.write_paged_kv`);
+        of each request, its query tokens' own included (see :func:`dkernel_b200.write_paged_kv`), or is 0 for
+        an idle request, whose query tokens attend nothing;
         ``cu_seqlen_q`` (batch + 1,) says whose the query tokens are (None: one each).  The last tokens of a
         request are its queries: a chain, or with ``tree_mask`` a tree of at most 64 drafted tokens, where
         bit j of the 64-bit word ``tree_mask[t]`` says that query t attends draft j of its request (its

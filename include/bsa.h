@@ -419,8 +419,9 @@ int bsa_paged_write(const bsa_paged_write_params* p, void* stream);
  * of head h attends
  *   context token s           iff the pattern has block (pos_i / bs, s / bs),
  *   draft j that its mask has iff the pattern has block (pos_i / bs, pos_j / bs).
- * A row that attends nothing: o = 0, lse = -inf.  Rows of q behind cu_q[batch]
- * are left alone.  Every query that an entry does not attend is independent of
+ * A row that attends nothing: o = 0, lse = -inf.  So are the rows of a request
+ * that stores nothing (seqlens[b] <= 0), whatever its table names; otherwise
+ * seqlens[b] >= n.  Rows of q behind cu_q[batch] are left alone.  Every query that an entry does not attend is independent of
  * it, whatever the entry's keys and values hold (infinities and NaN included). */
 typedef struct {
   const void* q; void* o; float* lse;   /* (total_q, hq, d) x 2, (hq, total_q) or NULL  */

@@ -173,8 +173,9 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(bsa_paged_step
         p.block_tables[(int64_t)b * p.table_stride + i] = popped(off[b] + i - held[b]);
   if (rank == 0) {
     for (int b = tid; b < B; b += kStepThreads) {
+      // written where it stays, too: a count outside [0, W] has been clamped, and the slots' kernel reads it here
       const int h = held[b], tg = target[b];
-      if (tg != h) p.page_counts[b] = tg < h ? tg : h + min(max(avail - off[b], 0), tg - h);
+      p.page_counts[b] = tg <= h ? tg : h + min(max(avail - off[b], 0), tg - h);
     }
     if (tid == 0) {
       *p.num_free = max(avail - pops, 0);

@@ -37,3 +37,27 @@ def test_requests_that_store_nothing(impl, kind, fp8):
                                kv_scales=x["kv_scales"] or (1.0, 1.0))
     assert torch.equal(torch.isinf(lse).cpu(), torch.isinf(ref_lse))
     assert (out.cpu().double() - ref).abs().max() < 0.02
+
+
+@pytest.mark.parametrize("tokens", [4096, 6000])
+def test_page_counts_outside_the_table(tokens):
+    """Counts that no step wrote, past the table's width or negative: the request holds its whole row, or nothing, and no
+    token gets a slot of its neighbour's, in the step of one launch and in that of two."""
+    from dkernel_b200 import plan_paged_step
+    i32 = dict(dtype=torch.int32, device="cuda")
+    page, W = 16, 4
+    table = torch.arange(3 * W, **i32).view(3, W).contiguous()
+    table[1] = -1
+    counts = torch.tensor([9, -5, W + 1], **i32)
+    stack, top = torch.arange(100, 110, **i32), torch.tensor([10], **i32)
+    ctx, new = [10, 0, 63], [2000, 20, 2000]
+    got = plan_paged_step(table, counts, stack, top, torch.tensor(ctx, **i32), torch.tensor(new, **i32), page_size=page,
+                          max_new_tokens=tokens)
+    assert counts.tolist() == [W, 2, W] and top.item() == 8 and got.short.item() == 0
+    assert table.tolist() == [[0, 1, 2, 3], [109, 108, -1, -1], [8, 9, 10, 11]]
+    want = []
+    for b, pages in enumerate(table.tolist()):
+        for i in range(new[b]):
+            at = ctx[b] + i
+            want.append(pages[at // page] * page + at % page if at < W * page and pages[at // page] >= 0 else -1)
+    assert got.slots.tolist() == want + [-1] * (tokens - len(want))

@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(256) paged_commit_kernel(bsa_paged_commit_para
     word = ((uint64_t)__ldg(p.tree_mask + t0 + a) & low_bits(n)) | 1ull << a;
   }
   const int count = !any ? 0 : p.tree_mask ? __popcll(word) : a + 1;
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.new_context_lens[b] = L + count;
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.new_context_lens[b] = (int)min((long long)L + count, 0x7fffffffll);
   if (!p.tree_mask || !any) return;   // a chain is in place already
   const int stay = __ffsll((long long)~word) - 1;   // the first drafts 0, 1, ... are, too (-1: all 64)
   if (stay < 0 || stay >= count) return;
@@ -319,10 +319,12 @@ __global__ void __launch_bounds__(256) paged_commit_kernel(bsa_paged_commit_para
     const int y = is_v ? x - per_cache : x, h = y / pieces, c = y - h * pieces;
     char* base = static_cast<char*>(is_v ? p.v_cache : p.k_cache);
     const int64_t sp = is_v ? p.vc_sp : p.kc_sp, ss = is_v ? p.vc_ss : p.kc_ss, sh = is_v ? p.vc_sh : p.kc_sh;
-    auto place = [&](int at) -> V* {
-      const int pg = page_of(table, at / p.page_size, p.max_pages, p.num_pages);
+    // unsigned: L + 63 may pass 2^31, and a negative page would be looked up in front of the table
+    auto place = [&](uint32_t at) -> V* {
+      const uint32_t pi = at / (uint32_t)p.page_size;
+      const int pg = page_of(table, pi, p.max_pages, p.num_pages);
       if (pg < 0) return nullptr;
-      return reinterpret_cast<V*>(base + ((int64_t)pg * sp + (int64_t)(at % p.page_size) * ss + (int64_t)h * sh) * elem_bytes) + c;
+      return reinterpret_cast<V*>(base + ((int64_t)pg * sp + (int64_t)(at - pi * (uint32_t)p.page_size) * ss + (int64_t)h * sh) * elem_bytes) + c;
     };
     uint64_t left = word & ~low_bits(stay);
     int r = stay;
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(256) paged_commit_kernel(bsa_paged_commit_para
       for (int i = 0; i < 4; ++i) {
         src[i] = nullptr;
         if (!left) continue;
-        src[i] = place(L + __ffsll((long long)left) - 1);
+        src[i] = place((uint32_t)L + (uint32_t)(__ffsll((long long)left) - 1));
         left &= left - 1;
         if (src[i]) val[i] = *src[i];
         ++m;
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(256) paged_commit_kernel(bsa_paged_commit_para
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i >= m) continue;
-        V* dst = place(L + r + i);
+        V* dst = place((uint32_t)L + (uint32_t)(r + i));
         if (src[i] && dst) *dst = val[i];
       }
       r += m;

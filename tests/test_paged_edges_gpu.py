@@ -61,3 +61,20 @@ def test_page_counts_outside_the_table(tokens):
             at = ctx[b] + i
             want.append(pages[at // page] * page + at % page if at < W * page and pages[at // page] >= 0 else -1)
     assert got.slots.tolist() == want + [-1] * (tokens - len(want))
+
+
+def test_commit_behind_every_page():
+    """Context lengths up to the largest int32, where no page is: nothing moves, lengths saturate."""
+    from dkernel_b200 import commit_paged_draft
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for page in (1, 16):
+        k, v = (torch.randn((4, page, 2, 64), device="cuda").to(bf16) for _ in range(2))
+        keep = [k.clone(), v.clone()]
+        table = torch.arange(4, **i32)[None].repeat(3, 1)
+        ctx = torch.tensor([2 ** 31 - 1, 2 ** 31 - 20, -7], **i32)
+        n = 64
+        words = P.as_int64([(1 << 64) - 2 if j == 63 else 1 << j for j in range(n)] * 3).cuda()
+        acc = torch.tensor([63, 63, -1], **i32)
+        lens = commit_paged_draft(k, v, table, ctx, torch.tensor([0, n, 2 * n, 3 * n], **i32), acc, tree_mask=words)
+        assert lens.tolist() == [2 ** 31 - 1, 2 ** 31 - 1, 0]
+        assert torch.equal(k, keep[0]) and torch.equal(v, keep[1])

@@ -304,6 +304,14 @@ _DYNAMIC_TILES_FROM = 1024     # 128-row tiles from which a forward launch gets 
 _DS_WS_MAX_BYTES = 8 << 30     # largest dS scratch the backward allocates by itself
 
 
+def _warn_fallback(why: bytes, stacklevel: int) -> None:
+    if why not in _warned_fallback:
+        _warned_fallback.add(why)
+        import warnings
+        warnings.warn("dkernel_b200: this attention call runs on the CUDA-core fallback kernel, "
+                      f"not on the tensor cores: {why.decode()}", RuntimeWarning, stacklevel=stacklevel)
+
+
 def _launch_fwd(p, q: Tensor) -> None:
     """bsa_fwd on q's device and stream.  A call whose shape the tensor-core kernel handles but
     which would still run on the CUDA-core kernel (an unaligned output view, for instance) is
@@ -313,11 +321,8 @@ def _launch_fwd(p, q: Tensor) -> None:
     if (p.impl != _lib.IMPL_GENERIC and p.dtype != _lib.BSA_F32 and p.d % 8 == 0 and p.d <= 256
             and p.block_size == 64):
         why = lib.bsa_fwd_why_not_sm100(C.byref(p))
-        if why and p.impl == _lib.IMPL_AUTO and why not in _warned_fallback:
-            _warned_fallback.add(why)
-            import warnings
-            warnings.warn("dkernel_b200: this attention call runs on the CUDA-core fallback kernel, "
-                          f"not on the tensor cores: {why.decode()}", RuntimeWarning, stacklevel=3)
+        if why and p.impl == _lib.IMPL_AUTO:
+            _warn_fallback(why, 4)
         rows = p.total_q if p.total_q > 0 else p.batch * p.sq
         if not why and rows * p.hq >= _DYNAMIC_TILES_FROM * 128:
             # more tiles than a few rounds of the persistent grid: let the CTAs draw them from a
@@ -772,6 +777,11 @@ def _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, tabl
     if need:
         ws = q.new_empty(need, dtype=torch.uint8)
         p.ws = ws.data_ptr()
+    elif impl == _lib.IMPL_AUTO and code != _lib.BSA_F32 and d <= 256 and pages > 0 and tables.size(1) > 0:
+        # no workspace: not the tensor-core kernel.  A 16-bit call that is a hundred times slower is reported, once per reason
+        why = lib.bsa_paged_why_not_sm100(C.byref(p))
+        if why:
+            _warn_fallback(why, 4)
     _lib.launch(lib.bsa_paged_fwd, p, dev, "bsa_paged_fwd")
     return o, lse
 

@@ -78,3 +78,31 @@ def test_commit_behind_every_page():
         lens = commit_paged_draft(k, v, table, ctx, torch.tensor([0, n, 2 * n, 3 * n], **i32), acc, tree_mask=words)
         assert lens.tolist() == [2 ** 31 - 1, 2 ** 31 - 1, 0]
         assert torch.equal(k, keep[0]) and torch.equal(v, keep[1])
+
+
+def test_calls_for_the_cuda_cores_say_so():
+    """16-bit calls that the tensor-core kernel does not serve are reported, once per reason; fp32, calls by name, and calls
+    without a page are not."""
+    import warnings
+    from dkernel_b200 import ops
+    pat = local_stride(2, 4, 2, 2)
+
+    def warned(d=64, dtype=bf16, page=16, fp8=False, impl="auto", width=None):
+        x = paged_inputs(1, 4, 2, d, [70, 3], [5, 9], page, dtype, fp8=fp8)
+        if width is not None:
+            x["table"] = x["table"][:, :width]
+        with warnings.catch_warnings(record=True) as got:
+            warnings.simplefilter("always")
+            call(module(64, pat, seq_dim=1, impl=impl), x)
+        return [str(w.message) for w in got if issubclass(w.category, RuntimeWarning)]
+
+    keep = set(ops._warned_fallback)
+    try:
+        ops._warned_fallback.clear()
+        assert not warned() and not warned(dtype=torch.float32) and not warned(page=24, impl="generic") and not warned(width=0)
+        assert ["page size" in m for m in warned(page=24)] == [True]
+        assert not warned(page=24)
+        assert ["head dim" in m for m in warned(d=40, fp8=True)] == [True]
+    finally:
+        ops._warned_fallback.clear()
+        ops._warned_fallback.update(keep)

@@ -37,7 +37,11 @@ def _tma_friendly(t: Tensor) -> Tensor:
     bits = t.data_ptr()
     for s in st[:-1]:
         bits |= s * size
-    return t.contiguous() if bits & 15 else t
+    if not bits & 15:
+        return t
+    c = t.contiguous()
+    # a contiguous view that starts off the boundary is its own contiguous(); of odd head dims no copy is aligned
+    return c.clone() if c.data_ptr() & 15 and t.size(-1) * size % 16 == 0 else c
 
 
 def _empty_like(t: Tensor) -> Tensor:

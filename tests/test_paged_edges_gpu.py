@@ -6,7 +6,7 @@ import torch
 
 from oracle import paged_oracle as P
 from paged_cases import local_stride, paged_inputs
-from test_paged_gpu import call, module
+from test_paged_gpu import call, device, module
 
 pytestmark = pytest.mark.gpu
 bf16 = torch.bfloat16
@@ -106,3 +106,26 @@ def test_calls_for_the_cuda_cores_say_so():
     finally:
         ops._warned_fallback.clear()
         ops._warned_fallback.update(keep)
+
+
+def test_contiguous_tensors_off_the_16_byte_boundary():
+    """Slices of a larger buffer that are contiguous and start 2 bytes off are copied, not handed to the CUDA cores."""
+    pat = local_stride(2, 8, 2, 3)
+
+    def off(t):
+        flat = torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+
+    x = paged_inputs(8, 4, 2, 64, [100, 30], [20, 33], 16, bf16)
+    mod, c = module(64, pat, seq_dim=1, impl="sm100"), device(x)
+    want = call(mod, x, c)
+    q = off(c["q"])
+    assert q.data_ptr() % 16 == 2 and q.is_contiguous()
+    assert torch.equal(call(mod, x, {**c, "q": q}), want)
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn((2, 200, h, 64), generator=g).to(bf16).cuda() for h in (4, 2, 2))
+    with torch.no_grad():
+        assert torch.equal(mod(off(q), off(k), off(v)), mod(q, k, v))
+        last = [q[:, -1:].contiguous(), k, v]
+        assert torch.equal(mod(*map(off, last)), mod(*last))

@@ -129,3 +129,12 @@ def test_contiguous_tensors_off_the_16_byte_boundary():
         assert torch.equal(mod(off(q), off(k), off(v)), mod(q, k, v))
         last = [q[:, -1:].contiguous(), k, v]
         assert torch.equal(mod(*map(off, last)), mod(*last))
+
+
+def test_broadcast_queries():
+    """One query row for all heads, or for all tokens (stride 0), on the tensor-core kernel."""
+    pat = local_stride(2, 8, 2, 3)
+    x = paged_inputs(8, 4, 2, 64, [100, 30], [20, 33], 16, bf16)
+    mod, c = module(64, pat, seq_dim=1, impl="sm100"), device(x)
+    for q in (c["q"][:, :1].expand(-1, 4, -1), c["q"][:1].expand(53, -1, -1), c["q"][:1, :1].expand(53, 4, -1)):
+        assert torch.equal(call(mod, x, {**c, "q": q}), call(mod, x, {**c, "q": q.contiguous()}))

@@ -17,6 +17,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _Plan, _paged_forward, _sparse_attention
@@ -170,9 +171,9 @@ class SparseAttention(torch.nn.Module):
         context's length plus the number of other drafts it attends.  Causal modules only; no gradients.
         Rows that attend nothing are 0 with LSE -inf; rows of ``out`` behind the last request stay as they
         are.  The LSE is (heads, tokens)."""
-        if block_tables is not None and k is not None and v is not None and not (
+        if block_tables is not None and k is not None and v is not None and forward_ad._current_level < 0 and not (
                 torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
-            # serving: nothing for autograd to record
+            # serving: nothing for autograd to record (inside a dual level it refuses tangents)
             return _paged_forward(self._plan(), self.kwargs, self.seq_dim, q, k, v, sm_scale, block_tables, seqlens,
                                   cu_seqlen_q, tree_mask, kv_scales, return_lse, cu_seqlen_k, left_paddings)
         inf_kwargs = {"cu_seqlen_k": cu_seqlen_k,

@@ -138,3 +138,20 @@ def test_broadcast_queries():
     mod, c = module(64, pat, seq_dim=1, impl="sm100"), device(x)
     for q in (c["q"][:, :1].expand(-1, 4, -1), c["q"][:1].expand(53, -1, -1), c["q"][:1, :1].expand(53, 4, -1)):
         assert torch.equal(call(mod, x, {**c, "q": q}), call(mod, x, {**c, "q": q.contiguous()}))
+
+
+def test_forward_mode_tangents_are_refused():
+    """There is no derivative: a tangent on q or the caches raises, as on the contiguous route, with and without no_grad."""
+    import torch.autograd.forward_ad as fwd
+    pat = local_stride(2, 8, 2, 3)
+    x = paged_inputs(8, 4, 2, 64, [100, 30], [20, 33], 16, bf16)
+    mod, c = module(64, pat, seq_dim=1), device(x)
+    want = call(mod, x, c)
+    with fwd.dual_level():
+        assert torch.equal(call(mod, x, c), want)
+        for name in ("q", "k", "v"):
+            dual = {**c, name: fwd.make_dual(c[name], torch.ones_like(c[name]))}
+            with pytest.raises(NotImplementedError):
+                call(mod, x, dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call(mod, x, dual)

@@ -1073,6 +1073,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               p.lse[(int64_t)head * p.lse_sh + pl->t0 + i_tok] = l > 0.f ? (m_used - kShift + log2f(l)) * kLn2 : -INFINITY;
             // an infinity or NaN got into the row: attended or not, the definition says what it is
             uint32_t redo = __ballot_sync(0xffffffffu, row_ok && l != 0.f && (check != 0.f || !(l > 0.f)));
+            __syncwarp();                     // other lanes write the row again
             while (redo) {
               const int src = __ffs(redo) - 1;
               redo &= redo - 1;
@@ -1334,6 +1335,7 @@ __device__ __forceinline__ void join_rows(const bsa_paged_params& p, const Paged
       if (p.lse && lane == 0) p.lse[(int64_t)h * p.lse_sh + t] = l[x] > 0.f ? (m[x] - shift + log2f(l[x])) * kLn2 : -INFINITY;
       if (__any_sync(0xffffffffu, bad) && l[x] != 0.f) redo |= 1u << x;
     }
+    __syncwarp();                                        // other lanes write these rows again
     while (redo) {
       const int row = row0 + __ffs(redo) - 1, tok = (int)((row + 0.5f) * sh.inv_gt);
       redo &= redo - 1;

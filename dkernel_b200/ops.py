@@ -717,9 +717,10 @@ def _paged_forward(plan, kwargs, seq_dim, q, k, v, sm_scale, block_tables, seqle
 
 def _paged_statics(plan: _Plan, q: Tensor, hq: int, hkv: int, impl: int) -> Tuple[int, ...]:
     """The layout fields of a paged call, which follow from the module and the head counts alone."""
-    key = (hq, hkv, impl, q.dtype, q.size(-1))
+    key = (hq, hkv, impl, q.dtype, q.size(-1), q.get_device())
     got = plan._paged.get(key)
     if got is None:
+        assert plan.crow.device == q.device, f"the module is on {plan.crow.device}, q is on {q.device}"
         n_pat = plan.crow.size(0)
         assert n_pat in (1, hkv, hq), f"q and the cache have ({hq}, {hkv}) heads, the sparse pattern has {n_pat}"
         kp = plan

@@ -128,3 +128,15 @@ def test_functions_refuse_cpu_tensors():
         write_paged_kv(k[0, :2], k[0, :2], k, k, z.long())
     with pytest.raises(RuntimeError, match="no CPU path"):
         commit_paged_draft(k, k, t, z, z, z)
+
+
+def test_modules_on_another_device_are_refused():
+    """The layouts' pointers are read on q's device."""
+    from dkernel_b200 import _lib
+    from dkernel_b200.ops import _Plan, _paged_statics
+    t = torch.zeros((1, 3), dtype=torch.int32)
+    q = torch.zeros((1, 2, 64), dtype=torch.bfloat16)
+    assert len(_paged_statics(_Plan(t, t, t, t, 64, 1), q, 2, 2, _lib.IMPL_AUTO)) == 8
+    m = t.to("meta")
+    with pytest.raises(AssertionError, match="the module is on meta"):
+        _paged_statics(_Plan(m, m, m, m, 64, 1), q, 2, 2, _lib.IMPL_AUTO)

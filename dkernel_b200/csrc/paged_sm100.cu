@@ -230,7 +230,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   // the joining kernel reads nothing before this grid has ended; its launch may be prepared
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (*reinterpret_cast<volatile int*>(wait_status) != 0) return;
+  if (*reinterpret_cast<volatile int*>(wait_status) != 0) {
+    // what follows in the stream follows the kernel in front of this one, too (which may have let this one start early)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const int tid = threadIdx.x, lane = tid & 31;
   const int cta = blockIdx.x;
   const int warp = tid >> 5;

@@ -155,3 +155,45 @@ def test_forward_mode_tangents_are_refused():
                 call(mod, x, dual)
             with torch.no_grad(), pytest.raises(NotImplementedError):
                 call(mod, x, dual)
+
+
+def test_a_wait_that_gave_up_stops_the_kernels_and_not_the_stream():
+    """While the status word is set the attention call raises and writes nothing, and what follows it in the stream still
+    follows what was in front of it; clearing the word restores service."""
+    from dkernel_b200 import _lib, plan_paged_step
+    pat = local_stride(2, 8, 2, 3)
+    x = paged_inputs(8, 4, 2, 64, [100, 30], [20, 33], 16, bf16)
+    out = torch.empty((53, 4, 64), dtype=bf16, device="cuda")
+    mod, c = module(64, pat, seq_dim=1, impl="sm100", out=out), device(x)
+    want = call(mod, x, c).clone()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    B, W, page = 4000, 40, 16
+
+    def state():
+        return [torch.full((B, W), -1, **i32), torch.zeros(B, **i32), torch.arange(B * W, **i32), torch.tensor([B * W], **i32)]
+
+    lens = torch.full((B,), W * page - 1, **i32)
+    new = torch.ones(B, **i32)
+    ref = state()
+    ref_step = plan_paged_step(*ref, lens, new, page_size=page, max_new_tokens=B)
+    torch.cuda.synchronize()
+    assert _lib.wait_status() == 0
+    assert _lib.lib().bsa_selftest_wait_timeout(1000, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    code = _lib.wait_status(reset=False)
+    assert code != 0
+    out.fill_(7.0)
+    got = state()
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.BsaError):
+        # the step's kernel lets its successor start early
+        plan_paged_step(*got, lens, new, page_size=page, max_new_tokens=B)
+    with pytest.raises(_lib.BsaError):
+        call(mod, x, c)
+    after = [t.clone() for t in got]
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+    assert all(torch.equal(a, r) for a, r in zip(after, ref))
+    assert _lib.wait_status() == code and _lib.wait_status() == 0
+    assert torch.equal(call(mod, x, c), want)
+    assert ref_step.short.item() == 0

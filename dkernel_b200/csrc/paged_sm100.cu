@@ -2,7 +2,7 @@
 // their type or e4m3; head dims that are multiples of 8, 16 for e4m3, up to 128; pattern blocks of 16, 32 or 64
 // tokens; pages of a power of two of tokens, 8 or more).  Semantics: include/bsa.h.
 //
-// What bounds it: every attended K/V byte of a (request, kv head) has to come from HBM once.  An ITEM is a tile of
+// What it cannot do without: every attended K/V byte of a (request, kv head) has to come from HBM once.  An ITEM is a tile of
 // 128 rows = drafted tokens x q heads of a kv group, and the pattern blocks that any of them attends.  The items' blocks
 // are shared out over two persistent CTAs per SM in equal pieces, whatever the requests' lengths: a CTA's piece may begin
 // and end inside an item, whose partial results a second kernel then joins.  Requests with more rows than a tile have
@@ -23,8 +23,11 @@
 // 22 us.  A launch's first 9 us go by until its first tile is there: tables and lists, each instruction met for the first
 // time; then single tokens run at what HBM gives, wide trees at the pace of the softmax warps (two per scheduler: 1850
 // cycles a tile against 1024 of exponentials), with shared memory three quarters busy (Q, K and twice V as operands).
-// The cost of a join: 2 to 8 us.  K/V tiles pass through L2 evict-first: without that this code and the tables are fetched
-// from DRAM again, launch after launch, and trees take 10 % more.
+// That pace is two thirds of the trees' time and half of the e4m3 trees'; what the rest waits for is not known.  An e4m3 cache
+// makes calls slower, not faster: the same 64 single tokens 103 us against 84, the trees 150 against 108, the wide trees 201
+// against 142; two warps expand each of its tiles in shared memory before the products.  The cost of a join: 2 to 8 us.  K/V
+// tiles pass through L2 evict-first: without that this code and the tables are fetched from DRAM again, launch after launch,
+// and trees take 10 % more.
 #include <type_traits>
 
 #include "ptx.cuh"
@@ -134,8 +137,9 @@ template <bool BF16> __device__ __forceinline__ uint32_t ppack2(float lo, float 
     return *reinterpret_cast<uint32_t*>(&h);
   }
 }
-// p = hi + lo, hi cut off (what it leaves is at most 2^-8 of p and is kept to 2^-9 of that).  An infinity in V meets a
-// low term of 0 here and gives NaN; such rows are computed again.
+// p = hi + lo, hi cut off: it leaves at most 2^-7 of p in bf16, 2^-10 in f16, and lo's rounding 2^-16 and 2^-22 of p.  As
+// two_terms, but without its least low term: an infinity in V meets a low term of 0 here and gives NaN; such rows are
+// computed again.
 template <bool BF16> __device__ __forceinline__ void psplit(float p0, float p1, uint32_t& hi, uint32_t& lo) {
   float h0, h1, l0, l1;
   if (BF16) {
@@ -196,7 +200,8 @@ __device__ __forceinline__ Entry entry_of(const PagedShape& sh, int e, int nE, i
   Entry x;
   x.half = e >= nE;
   const int y = x.half ? e - nE : e;
-  x.b = nE < (1 << 20) ? (int)((y + 0.5f) * sh.inv_hkv) : y / hkv;     // exact: (y + 1/2) / hkv is 1/16 off an integer at least
+  // exact: (y + 1/2) / hkv is 1 / (2 hkv) off an integer at least; the product's error is 2^-23 of less than 2^20 / hkv
+  x.b = nE < (1 << 20) ? (int)((y + 0.5f) * sh.inv_hkv) : y / hkv;
   x.kvh = y - x.b * hkv;
   return x;
 }
@@ -469,7 +474,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           PagedRec rec = {1, b, r.t0, r.n, r.L, tok0, ntok, head0, gcnt, (int)div(item0 + n0, (int)min(share, 0x7fffffffll))};
           recs[cta] = rec;
         }
-        // up to 16 rows are repeated; more would cost more at the item's end than the repetitions save at its tiles
+        // up to 16 rows are repeated (repetitions of 32 and 64 rows, with more to add up at the item's end, were not built)
         const int rr = sh.cr == 16 && ntok <= sh.ct ? 16 : 128;
         n = 0;
         bool first = true, begins = true;
@@ -1375,7 +1380,8 @@ void plan_shape(const bsa_paged_params* p, PagedShape* sh) {
   }
   sh->gt = gt;
   sh->chunks = cdiv_i(G, gt);
-  // chunks of 16 rows where a tile holds no fewer tokens with them than in chunks of 32
+  // chunks of 16 rows where a tile holds no fewer tokens with them than in chunks of 32.  Single tokens, 64 requests over
+  // 1024..8192 tokens: groups of 4 and 8 heads (16 rows, repeated) 84.0 and 87.5 us, of 6 and 10 (32, not repeated) 85.2, 85.8
   sh->cr = gt <= 16 && 2 * (16 / gt) >= 32 / gt ? 16 : gt <= 32 ? 32 : gt <= 64 ? 64 : 128;
   sh->ct = p->cu_q ? sh->cr / gt : 1;      // single tokens: the rows behind them stay zeros
   sh->tt = 128 / sh->cr * sh->ct;

@@ -357,8 +357,8 @@ _IMPL_NAMES = {None: _lib.IMPL_AUTO, "auto": _lib.IMPL_AUTO, "generic": _lib.IMP
 
 
 def _fp8_kv_scales(q: Tensor, k: Tensor, kv_scales) -> Optional[Tuple[float, float]]:
-    """The (k_scale, v_scale) of an e4m3 K/V cache, or None for K/V of q's type.  Only the decode
-    kernel reads 8-bit K/V: a single query token per sequence on 64/128-wide heads."""
+    """The (k_scale, v_scale) of an e4m3 K/V cache, or None for K/V of q's type.  8-bit K/V are read by the
+    decode kernel (a single query token per sequence on 64/128-wide heads) and from paged caches."""
     if _FP8 is None or k.dtype != _FP8:
         assert kv_scales is None, "kv_scales only applies to float8_e4m3fn K/V"
         return None

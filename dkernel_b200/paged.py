@@ -14,7 +14,9 @@ One step of a server that drafts tokens (speculative decoding)::
                                       accepted, tree_mask=tree_mask)
 
 Everything stays on the device and runs on the current stream; nothing synchronises, so a step can be captured
-into a CUDA graph.  Pages of different requests are distinct, as ``plan_paged_step`` hands them out.
+into a CUDA graph, once each call has been made outside a capture: a module's first one with given head counts reads
+its pattern from the device (a pattern per query head) or refines it (blocks of 128 tokens), and keeps the result.
+Pages of different requests are distinct, as ``plan_paged_step`` hands them out.
 """
 from __future__ import annotations
 
@@ -34,7 +36,7 @@ class PagedStep(NamedTuple):
     seqlens: Tensor         # (batch,) int32: stored tokens per request, the new ones included
     slots: Tensor           # (max_new_tokens,) int64: where each new token's K and V go; -1 = nowhere
     positions: Tensor       # (max_new_tokens,) int32: each new token's position in its sequence
-    short: Tensor           # (1,) int32: pages that were missing, 0 when all is well
+    short: Tensor           # (1,) int32: pages that the stack could not give; see plan_paged_step for tables that are too narrow
 
 
 def _state32(t: Tensor, shape: Optional[Tuple[int, ...]], device_index: int, name: str) -> Tensor:
@@ -56,7 +58,9 @@ def plan_paged_step(block_tables: Tensor, page_counts: Tensor, free_pages: Tenso
     Updated in place, all int32: ``block_tables`` (batch, pages per request), ``page_counts`` (batch,),
     ``free_pages`` (any size that holds all pages), ``num_free`` (1,).  Where the stack runs empty the table gets -1,
     the tokens have slot -1 (their keys and values are stored nowhere) and ``short`` counts the missing pages; a later step
-    with the same lengths gets them once pages are free.
+    with the same lengths gets them once pages are free.  No page helps a request that has outgrown its row of the table:
+    its tokens past the row have slot -1, too, and are not counted in ``short``; such requests are those with
+    ``seqlens > block_tables.size(1) * page_size``.
     ``max_new_tokens`` is the size of the packed batch: outputs behind the last request are slot -1, position 0, and
     new tokens past it are dropped.  With ``tree_mask`` (max_new_tokens,) int64, see ``SparseAttention.forward``, a
     position is the context's length plus the number of other drafts attended, else they count up."""
@@ -135,7 +139,9 @@ def commit_paged_draft(k_cache: Tensor, v_cache: Tensor, block_tables: Tensor, c
     ``accepted[b]`` is the number of the last accepted draft of request b (-1, or any number that is not one of its
     drafts: none).  Its branch is the drafts that it attends under ``tree_mask``, and itself (without ``tree_mask``
     drafts 0..accepted[b]); their keys and values move, in the order of their numbers, to the places right behind the
-    context.  The other drafts' slots hold leftovers afterwards.  Returns the new context lengths (int32, a new tensor;
+    context.  The other drafts' slots hold leftovers afterwards.  Every token of the branch needs its page: one whose slot
+    was -1 in the step is stored nowhere, so nothing moves to its place behind the context, which keeps what lay there, and
+    it counts in the new length all the same.  Accept nothing for a request that the step left without a page.  Returns the new context lengths (int32, a new tensor;
     ``context_lens`` stays as it is).  Positions do not change, so rotated keys need nothing further."""
     seq_dim = 1 if seq_dim is None else seq_dim
     assert seq_dim in (1, 2)

@@ -366,7 +366,8 @@ int bsa_xchg_merge(const bsa_xchg_params* p, void* stream);
  * afterwards (at most max_pages).  Surplus pages of all requests are pushed on
  * the stack free_pages[0 .. num_free) in the order (request, page), then the
  * missing ones are popped from its top in that order; where the stack runs
- * empty the table gets -1 and *short_pages counts the pages that were missing.
+ * empty the table gets -1 and *short_pages counts the pages that were missing
+ * (pages past max_pages are not counted: seqlens[b] > max_pages * page_size).
  * A request with no context and no new tokens gives back all it holds.
  * block_tables, page_counts, free_pages and num_free are updated in place.
  * Negative lengths count as 0; new tokens past max_tokens in all are dropped. */
@@ -452,7 +453,9 @@ const char* bsa_paged_why_not_sm100(const bsa_paged_params* p);
  * the branch of draft a = accepted[b] is the drafts that a attends and a itself
  * (without tree_mask drafts 0..a), in the order of their numbers; its r-th one
  * moves from logical token L + j to L + r in both caches, and
- * new_context_lens[b] = L + length of the branch.  accepted[b] outside [0, n),
+ * new_context_lens[b] = L + length of the branch.  A branch token without a page
+ * does not move and leaves its new place as it is, but counts in the length:
+ * accept nothing for requests whose step left them without one.  accepted[b] outside [0, n),
  * or past 63 with tree_mask: nothing is accepted.  L = context_lens[b], n as in bsa_paged_params. */
 typedef struct {
   void* k_cache; void* v_cache;

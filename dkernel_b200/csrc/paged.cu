@@ -117,14 +117,14 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(bsa_paged_step
   const int rank = blockIdx.x;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int n_free = min(max(__ldg(p.num_free), 0), p.free_capacity);
+  const int n_free = min(max(*p.num_free, 0), p.free_capacity);     // this and the counts are written below: no __ldg
   long long new_before = 0, moved_before = 0;
   if (tid == 0) cu[0] = 0;
   for (int b0 = 0; b0 < B; b0 += kStepThreads) {
     const int b = b0 + tid;
     const int want = b < B ? max(__ldg(p.new_lens + b), 0) : 0;
     const int ctx = b < B ? max(__ldg(p.context_lens + b), 0) : 0;
-    const int h = b < B ? min(max(__ldg(p.page_counts + b), 0), W) : 0;
+    const int h = b < B ? min(max(p.page_counts[b], 0), W) : 0;
     long long total;
     const long long incl = block_scan(want, warp_sums, &total) + new_before;
     const int c1 = (int)min(incl, (long long)T), c0 = (int)min(incl - want, (long long)T);

@@ -13,16 +13,18 @@ struct PagedRequest { int t0, n, L; bool stored = true; };
 // Query rows stay inside [0, total_q) whatever cu_q holds.  A request that stores nothing has rows that attend nothing
 // (batches are padded with such requests); one that stores some tokens, but fewer than it queries, counts as one without
 // context.
+// Tables, lengths and mask words are loaded as data that may have changed since the launch (no __ldg): the tensor-core
+// kernel may be resident before the step's kernel in front of it has written them.
 __device__ __forceinline__ PagedRequest paged_request(const bsa_paged_params& p, int b) {
   PagedRequest r;
   if (p.cu_q) {
-    r.t0 = min(max(__ldg(p.cu_q + b), 0), p.total_q);
-    r.n = min(max(__ldg(p.cu_q + b + 1) - r.t0, 0), p.total_q - r.t0);
+    r.t0 = min(max(p.cu_q[b], 0), p.total_q);
+    r.n = min(max(p.cu_q[b + 1] - r.t0, 0), p.total_q - r.t0);
   } else {
     r.t0 = b;
     r.n = 1;
   }
-  const int stored = __ldg(p.seqlens + b);
+  const int stored = p.seqlens[b];
   r.stored = stored > 0;
   r.L = max(stored - r.n, 0);
   return r;
@@ -32,7 +34,7 @@ __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : (
 
 // The drafts (of the n of its request) that draft i attends, as far as a word can name them.
 __device__ __forceinline__ uint64_t draft_word(const bsa_paged_params& p, const PagedRequest& r, int i) {
-  return (uint64_t)__ldg(p.tree_mask + r.t0 + i) & low_bits(r.n);
+  return (uint64_t)p.tree_mask[r.t0 + i] & low_bits(r.n);
 }
 __device__ __forceinline__ int draft_depth(uint64_t word, int i) {
   return __popcll(i < 64 ? word & ~(1ull << i) : word);
@@ -41,7 +43,7 @@ __device__ __forceinline__ int draft_depth(uint64_t word, int i) {
 // Page of logical token s, or -1.
 __device__ __forceinline__ int page_of(const int32_t* table, int64_t page_index, int max_pages, int num_pages) {
   if (page_index >= max_pages) return -1;
-  const int pg = __ldg(table + page_index);
+  const int pg = table[page_index];
   return pg >= 0 && pg < num_pages ? pg : -1;
 }
 

@@ -197,3 +197,31 @@ def test_a_wait_that_gave_up_stops_the_kernels_and_not_the_stream():
     assert _lib.wait_status() == code and _lib.wait_status() == 0
     assert torch.equal(call(mod, x, c), want)
     assert ref_step.short.item() == 0
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_attention_right_behind_the_step(tokens):
+    """The step's tables are read by a kernel that may be resident before they are written: pages change hands in every
+    step, and the attention call behind it gives what it gives after a synchronisation."""
+    from dkernel_b200 import plan_paged_step
+    hq, hkv, d, bs, page, B, W = 8, 2, 64, 64, 16, 48, 40
+    pat = local_stride(hkv, 10, 3, 4)
+    mod = module(bs, pat, seq_dim=1, impl="sm100")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(4)
+    pages = B * W
+    k, v = (torch.randn((pages, page, hkv, d), generator=g).to(bf16).cuda() for _ in range(2))
+    q = torch.randn((B * tokens, hq, d), generator=g).to(bf16).cuda()
+    table, counts = torch.full((B, W), -1, **i32), torch.zeros(B, **i32)
+    free, top = torch.randperm(pages, generator=g).to(torch.int32).cuda(), torch.tensor([pages], **i32)
+    new = torch.full((B,), tokens, **i32)
+    lens = torch.randint(0, W * page - tokens, (60, B), generator=g).to(torch.int32).cuda()
+    lens[::3] = 0
+    torch.cuda.synchronize()
+    for it in range(60):
+        st = plan_paged_step(table, counts, free, top, lens[it], new, page_size=page, max_new_tokens=B * tokens)
+        kw = dict(block_tables=table, seqlens=st.seqlens, cu_seqlen_q=None if tokens == 1 else st.cu_seqlen_q, return_lse=True)
+        got = mod(q, k, v, **kw)
+        torch.cuda.synchronize()
+        want = mod(q, k, v, **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), it

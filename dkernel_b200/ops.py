@@ -754,10 +754,10 @@ def _paged(q, k, v, sm_scale, plan, seq_dim, causal, out, impl, return_lse, tabl
     k_scale, v_scale, kv_code = (*fp8, _lib.BSA_F8E4M3) if fp8 is not None else (1.0, 1.0, code)
     statics = _paged_statics(plan, q, hq, hkv, impl)
     # strides and alignment that TMA takes; a head past the next token's would make the tensor map's strides descend, and
-    # one query for all heads needs rows of its own for each
+    # one query for all heads or tokens needs rows of its own for each
     q = _tma_friendly(q)
     q_st, q_sh, _ = q.stride()
-    if q_st < q_sh or (q_sh == 0 and hq > 1):
+    if q_st < q_sh or q_st == 0 or q_sh == 0:
         q = q.contiguous()
         q_st, q_sh, _ = q.stride()
     if out is None:

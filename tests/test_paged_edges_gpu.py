@@ -138,6 +138,10 @@ def test_broadcast_queries():
     mod, c = module(64, pat, seq_dim=1, impl="sm100"), device(x)
     for q in (c["q"][:, :1].expand(-1, 4, -1), c["q"][:1].expand(53, -1, -1), c["q"][:1, :1].expand(53, 4, -1)):
         assert torch.equal(call(mod, x, {**c, "q": q}), call(mod, x, {**c, "q": q.contiguous()}))
+    x = paged_inputs(8, 1, 1, 64, [100, 30], [20, 33], 16, bf16)
+    mod, c = module(64, pat[:1], seq_dim=1, impl="sm100"), device(x)
+    q = c["q"].as_strided((53, 1, 64), (0, 0, 1))
+    assert torch.equal(call(mod, x, {**c, "q": q}), call(mod, x, {**c, "q": q.contiguous()}))
 
 
 def test_forward_mode_tangents_are_refused():
